@@ -33,6 +33,7 @@ CF_DEVERR_BLOCK_ID = 0x1
 CF_DEVERR_SLOT = 0x2
 CF_DEVERR_CONTEXT_LEN = 0x4
 CF_DEVERR_TIMEOUT = 0x8
+CF_DEVERR_POSITION = 0x10
 
 CF_STATIC_SCRATCH_BYTES = 16 << 20
 
@@ -81,6 +82,37 @@ class PrefillParams(ctypes.Structure):
         ("max_blocks_per_seq", c_int32),
         ("num_blocks", c_int64),
         ("dtype", c_int32),
+    ]
+
+
+class RopeParams(ctypes.Structure):
+    """cf_rope_params."""
+
+    _fields_ = [
+        ("query", c_void_p),
+        ("key", c_void_p),
+        ("value", c_void_p),
+        ("query_out", c_void_p),
+        ("key_out", c_void_p),
+        ("positions", c_void_p),
+        ("cos_sin", c_void_p),
+        ("query_weight", c_void_p),
+        ("key_weight", c_void_p),
+        ("query_stride", c_int64 * 2),
+        ("key_stride", c_int64 * 2),
+        ("value_stride", c_int64 * 2),
+        ("query_out_stride", c_int64 * 2),
+        ("key_out_stride", c_int64 * 2),
+        ("num_tokens", c_int32),
+        ("num_heads", c_int32),
+        ("num_kv_heads", c_int32),
+        ("head_dim", c_int32),
+        ("rotary_dim", c_int32),
+        ("max_positions", c_int32),
+        ("eps", c_float),
+        ("interleaved", c_int32),
+        ("dtype", c_int32),
+        ("weight_dtype", c_int32),
     ]
 
 
@@ -135,6 +167,27 @@ SIGNATURES = {
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32,
          c_int64, c_int32, c_void_p],
     ),
+    "cf_qk_norm_rope": (c_int32, [POINTER(RopeParams), c_void_p]),
+    "cf_rope_and_cache": (
+        c_int32, [POINTER(RopeParams), c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_void_p],
+    ),
+    "cf_rope_and_cache_fp8": (
+        c_int32,
+        [POINTER(RopeParams), c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_float, c_float, c_void_p],
+    ),
+    "cf_rope_and_cache_fp8_block": (
+        c_int32,
+        [POINTER(RopeParams), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_void_p],
+    ),
+    "cf_reshape_and_cache_fp8_block": (
+        c_int32,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32,
+         c_int64, c_int32, c_void_p],
+    ),
+    "cf_paged_attention_fp8_block_v1": (
+        c_int32, [POINTER(AttentionParams), c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],
+    ),
+    "cf_paged_attention_fp8_block_workspace_size": (c_size_t, [POINTER(AttentionParams)]),
     "cf_copy_blocks": (
         c_int32,
         [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int64, c_int32,

@@ -207,6 +207,64 @@ size_t v1_split_bytes(const cf_paged_attention_params* p, bool fp8_cache, int32_
   return (size_t)(2 * round(rows * 4) + round(rows * p->head_dim * 4));
 }
 
+// Shapes, types, strides and operands of the norm / rotation entry points.
+cf_status check_rope_params(const cf_rope_params* p, bool with_cache) {
+  if (p == nullptr) return CF_ERR_INVALID_ARGUMENT;
+  if (p->dtype != CF_F32 && p->dtype != CF_F16 && p->dtype != CF_BF16) return CF_ERR_INVALID_ARGUMENT;
+  if (p->weight_dtype != CF_F32 && p->weight_dtype != p->dtype) return CF_ERR_INVALID_ARGUMENT;
+  if (p->num_tokens < 0 || p->num_heads <= 0 || p->num_kv_heads <= 0 || p->head_dim <= 0 ||
+      p->rotary_dim < 2 || p->rotary_dim > p->head_dim || p->rotary_dim % 2 != 0 ||
+      p->max_positions <= 0 || p->interleaved < 0 || p->interleaved > 1)
+    return CF_ERR_INVALID_ARGUMENT;
+  if (p->head_dim % 2 != 0 || p->head_dim > 256) return CF_ERR_UNSUPPORTED;
+  // one head row of every kind fits an int32 count of rows per token
+  if ((int64_t)p->num_heads + 2 * (int64_t)p->num_kv_heads > 65535) return CF_ERR_UNSUPPORTED;
+  if ((p->query_weight || p->key_weight) && !(p->eps > 0.f && std::isfinite(p->eps)))
+    return CF_ERR_INVALID_ARGUMENT;
+  if (p->num_tokens == 0) return CF_OK;
+  const uintptr_t eb = dtype_bytes(p->dtype), wb = dtype_bytes(p->weight_dtype);
+  auto bad = [](const void* q, uintptr_t align) { return reinterpret_cast<uintptr_t>(q) % align != 0; };
+  if (!p->query || !p->key || !p->query_out || !p->positions || !p->cos_sin) return CF_ERR_INVALID_ARGUMENT;
+  if (with_cache ? !p->value : !p->key_out) return CF_ERR_INVALID_ARGUMENT;
+  if (bad(p->query, eb) || bad(p->key, eb) || bad(p->query_out, eb) || bad(p->cos_sin, 4) ||
+      bad(p->positions, 4) || bad(p->query_weight, wb) || bad(p->key_weight, wb) ||
+      bad(with_cache ? p->value : p->key_out, eb))
+    return CF_ERR_INVALID_ARGUMENT;
+  // no two rows of an output may meet (a stride of one row count is never used)
+  auto apart = [&](const int64_t* stride, int64_t heads) {
+    const bool h = heads == 1 || stride[1] >= p->head_dim || stride[1] <= -(int64_t)p->head_dim;
+    const bool t = p->num_tokens == 1 || stride[0] >= p->head_dim || stride[0] <= -(int64_t)p->head_dim;
+    return h && t;
+  };
+  if (!apart(p->query_out_stride, p->num_heads)) return CF_ERR_INVALID_ARGUMENT;
+  if (!with_cache && !apart(p->key_out_stride, p->num_kv_heads)) return CF_ERR_INVALID_ARGUMENT;
+  return CF_OK;
+}
+
+// The block-scaled caches' shapes.
+cf_status check_block_cache(int32_t head_dim, int32_t block_size, int64_t num_blocks) {
+  if (block_size <= 0 || num_blocks <= 0) return CF_ERR_INVALID_ARGUMENT;
+  if (block_size != 16 || head_dim % 16 != 0 || num_blocks > INT32_MAX / 16) return CF_ERR_UNSUPPORTED;
+  return CF_OK;
+}
+
+// Split of the block-scaled decode attention: partitions and their tokens, and
+// the workspace they take (0: unsplit).
+size_t block_split(const cf_paged_attention_params* p, int32_t* parts_out, int32_t* tokens_out) {
+  if (p->num_seqs <= 0) return 0;
+  constexpr int64_t kTargetCtas = 4 * 148;
+  const int64_t pairs = (int64_t)p->num_seqs * p->num_kv_heads;
+  int32_t split = 2048;
+  while (split > 256 && pairs * ((p->max_context_len + split - 1) / split) < kTargetCtas) split /= 2;
+  if (p->max_context_len <= split) return 0;
+  const int64_t parts = ((int64_t)p->max_context_len + split - 1) / split;
+  if (parts_out) *parts_out = (int32_t)parts;
+  if (tokens_out) *tokens_out = split;
+  const int64_t rows = (int64_t)p->num_seqs * p->num_heads * parts;
+  auto round = [](int64_t b) { return (b + 255) / 256 * 256; };
+  return (size_t)(2 * round(rows * 4) + round(rows * p->head_dim * 4));
+}
+
 }  // namespace
 }  // namespace cfb
 
@@ -406,6 +464,131 @@ cf_status cf_reshape_and_cache(const void* key, const void* value, void* key_cac
   return launch_reshape_and_cache(key, value, key_cache, value_cache, slot_mapping, num_tokens,
                                   num_kv_heads, (int64_t)head_dim * eb, block_size, nb,
                                   (cudaStream_t)stream);
+}
+
+cf_status cf_qk_norm_rope(const cf_rope_params* p, void* stream) {
+  const cf_status st = check_rope_params(p, /*with_cache=*/false);
+  if (st != CF_OK || p->num_tokens == 0) return st;
+  return launch_qk_norm_rope(*p, (cudaStream_t)stream);
+}
+
+cf_status cf_rope_and_cache(const cf_rope_params* p, void* key_cache, void* value_cache,
+                            const int32_t* slot_mapping, int32_t block_size, int64_t num_blocks,
+                            void* stream) {
+  cf_status st = check_rope_params(p, /*with_cache=*/true);
+  if (st != CF_OK) return st;
+  if (block_size <= 0 || num_blocks <= 0) return CF_ERR_INVALID_ARGUMENT;
+  if (num_blocks > INT64_MAX / block_size) return CF_ERR_INVALID_ARGUMENT;
+  if (p->num_tokens == 0) return CF_OK;
+  if (!key_cache || !value_cache || !slot_mapping) return CF_ERR_INVALID_ARGUMENT;
+  const uintptr_t eb = dtype_bytes(p->dtype);
+  if (reinterpret_cast<uintptr_t>(key_cache) % eb || reinterpret_cast<uintptr_t>(value_cache) % eb)
+    return CF_ERR_INVALID_ARGUMENT;
+  return launch_rope_and_cache(*p, key_cache, value_cache, slot_mapping, block_size, num_blocks, false, 1.f,
+                               1.f, (cudaStream_t)stream);
+}
+
+cf_status cf_rope_and_cache_fp8(const cf_rope_params* p, void* key_cache, void* value_cache,
+                                const int32_t* slot_mapping, int32_t block_size,
+                                int64_t num_blocks, float k_scale, float v_scale, void* stream) {
+  cf_status st = check_rope_params(p, /*with_cache=*/true);
+  if (st != CF_OK) return st;
+  if (block_size <= 0 || num_blocks <= 0) return CF_ERR_INVALID_ARGUMENT;
+  if (num_blocks > INT64_MAX / block_size) return CF_ERR_INVALID_ARGUMENT;
+  if (!(k_scale > 0.f) || !(v_scale > 0.f) || !std::isfinite(k_scale) || !std::isfinite(v_scale))
+    return CF_ERR_INVALID_ARGUMENT;
+  if (p->head_dim % 16 != 0) return CF_ERR_UNSUPPORTED;
+  if (p->num_tokens == 0) return CF_OK;
+  if (!key_cache || !value_cache || !slot_mapping || !aligned16(key_cache) || !aligned16(value_cache))
+    return CF_ERR_INVALID_ARGUMENT;
+  return launch_rope_and_cache(*p, key_cache, value_cache, slot_mapping, block_size, num_blocks, true,
+                               k_scale, v_scale, (cudaStream_t)stream);
+}
+
+cf_status cf_rope_and_cache_fp8_block(const cf_rope_params* p, void* key_cache, void* value_cache,
+                                      float* k_scales, float* v_scales,
+                                      const int32_t* slot_mapping, int32_t block_size,
+                                      int64_t num_blocks, void* stream) {
+  cf_status st = check_rope_params(p, /*with_cache=*/true);
+  if (st != CF_OK) return st;
+  st = check_block_cache(p->head_dim, block_size, num_blocks);
+  if (st != CF_OK || p->num_tokens == 0) return st;
+  if (!key_cache || !value_cache || !k_scales || !v_scales || !slot_mapping || !aligned16(key_cache) ||
+      !aligned16(value_cache))
+    return CF_ERR_INVALID_ARGUMENT;
+  return launch_rope_and_cache_fp8_block(*p, key_cache, value_cache, k_scales, v_scales, slot_mapping,
+                                         num_blocks, (cudaStream_t)stream);
+}
+
+cf_status cf_reshape_and_cache_fp8_block(const void* key, const void* value, void* key_cache,
+                                         void* value_cache, float* k_scales, float* v_scales,
+                                         const int32_t* slot_mapping, int32_t num_tokens,
+                                         int32_t num_kv_heads, int32_t head_dim,
+                                         int32_t block_size, int64_t num_blocks, int32_t dtype,
+                                         void* stream) {
+  if ((dtype != CF_F32 && dtype != CF_F16 && dtype != CF_BF16) || num_tokens < 0 ||
+      num_kv_heads <= 0 || head_dim <= 0)
+    return CF_ERR_INVALID_ARGUMENT;
+  if (head_dim > 256) return CF_ERR_UNSUPPORTED;
+  const cf_status st = check_block_cache(head_dim, block_size, num_blocks);
+  if (st != CF_OK || num_tokens == 0) return st;
+  if (!key || !value || !key_cache || !value_cache || !k_scales || !v_scales || !slot_mapping)
+    return CF_ERR_INVALID_ARGUMENT;
+  const uintptr_t eb = dtype_bytes(dtype);
+  if (reinterpret_cast<uintptr_t>(key) % eb || reinterpret_cast<uintptr_t>(value) % eb || !aligned16(key_cache) ||
+      !aligned16(value_cache))
+    return CF_ERR_INVALID_ARGUMENT;
+  cf_rope_params p = {};
+  p.key = key;
+  p.value = value;
+  p.key_stride[0] = p.value_stride[0] = (int64_t)num_kv_heads * head_dim;
+  p.key_stride[1] = p.value_stride[1] = head_dim;
+  p.num_tokens = num_tokens;
+  p.num_kv_heads = num_kv_heads;
+  p.head_dim = head_dim;
+  p.dtype = dtype;
+  p.weight_dtype = dtype;
+  return launch_rope_and_cache_fp8_block(p, key_cache, value_cache, k_scales, v_scales, slot_mapping,
+                                         num_blocks, (cudaStream_t)stream);
+}
+
+size_t cf_paged_attention_fp8_block_workspace_size(const cf_paged_attention_params* p) {
+  if (check_attention_params(p, /*check_pointers=*/false) != CF_OK) return 0;
+  if (check_fp8(p, 1.f, 1.f) != CF_OK || p->num_blocks <= 0) return 0;
+  // the most that any max_context_len up to this one takes
+  cf_paged_attention_params q = *p;
+  size_t bytes = 0;
+  for (int64_t c = 128;; c += 128) {
+    q.max_context_len = (int32_t)(c < p->max_context_len ? c : p->max_context_len);
+    const size_t b = block_split(&q, nullptr, nullptr);
+    bytes = b > bytes ? b : bytes;
+    if (c >= p->max_context_len) break;
+  }
+  return bytes;
+}
+
+cf_status cf_paged_attention_fp8_block_v1(const cf_paged_attention_params* p, const float* k_scales,
+                                          const float* v_scales, void* workspace,
+                                          size_t workspace_bytes, void* stream) {
+  cf_status st = check_attention_params(p);
+  if (st != CF_OK) return st;
+  if ((st = check_fp8(p, 1.f, 1.f)) != CF_OK || p->num_seqs == 0) return st;
+  if (!k_scales || !v_scales || p->num_blocks <= 0) return CF_ERR_INVALID_ARGUMENT;
+  if (p->num_blocks * (int64_t)p->num_kv_heads * p->block_size > INT32_MAX) return CF_ERR_UNSUPPORTED;
+  BlockScaledLaunch l{p, k_scales, v_scales, 0, 1, nullptr, nullptr, nullptr, (cudaStream_t)stream};
+  int32_t parts = 1, tokens = 0;
+  const size_t need = block_split(p, &parts, &tokens);
+  if (need > 0 && workspace != nullptr && workspace_bytes >= need) {
+    if (!aligned16(workspace)) return CF_ERR_INVALID_ARGUMENT;
+    const int64_t r4 = ((int64_t)p->num_seqs * p->num_heads * parts * 4 + 255) / 256 * 256;
+    uint8_t* w = static_cast<uint8_t*>(workspace);
+    l.part_tokens = tokens;
+    l.num_parts = parts;
+    l.part_max = reinterpret_cast<float*>(w);
+    l.part_sum = reinterpret_cast<float*>(w + r4);
+    l.part_out = reinterpret_cast<float*>(w + 2 * r4);
+  }
+  return launch_block_scaled_attention(l);
 }
 
 cf_status cf_copy_blocks(void* key_cache, void* value_cache, const int64_t* block_mapping,
@@ -644,6 +827,8 @@ cf_status cf_get_device_errors(int32_t device, uint32_t* flags, int32_t clear) {
   if (st == CF_OK) st = attention_read_errors(&bits, clear != 0);
   if (st == CF_OK) st = cache_ops_read_errors(&bits, clear != 0);
   if (st == CF_OK) st = prefill_read_errors(&bits, clear != 0);
+  if (st == CF_OK) st = rope_read_errors(&bits, clear != 0);
+  if (st == CF_OK) st = block_scaled_read_errors(&bits, clear != 0);
   cudaSetDevice(prev);
   *flags = bits;
   return st;

@@ -92,4 +92,32 @@ cf_status launch_reshape_and_cache_fp8(const void* key, const void* value, void*
                                        float k_scale, float v_scale, cudaStream_t stream);
 cf_status cache_ops_read_errors(uint32_t* bits, bool clear);
 
+// ---- norms, rotation and append (rope_cache.cu) ------------------------------
+cf_status launch_qk_norm_rope(const cf_rope_params& p, cudaStream_t stream);
+cf_status launch_rope_and_cache(const cf_rope_params& p, void* key_cache, void* value_cache,
+                                const int32_t* slot_mapping, int32_t block_size,
+                                int64_t num_blocks, bool fp8, float k_scale, float v_scale,
+                                cudaStream_t stream);
+// p.num_heads 0 and p.positions null: the append alone.
+cf_status launch_rope_and_cache_fp8_block(const cf_rope_params& p, void* key_cache,
+                                          void* value_cache, float* k_scales, float* v_scales,
+                                          const int32_t* slot_mapping, int64_t num_blocks,
+                                          cudaStream_t stream);
+cf_status rope_read_errors(uint32_t* bits, bool clear);
+
+// ---- decode attention over block-scaled e4m3 caches (block_scaled_attention.cu) ----
+struct BlockScaledLaunch {
+  const cf_paged_attention_params* p;
+  const float* k_scales;
+  const float* v_scales;
+  int32_t part_tokens;  // tokens per partition (num_parts > 1)
+  int32_t num_parts;    // 1: unsplit
+  float* part_max;      // [num_seqs, num_heads, num_parts]
+  float* part_sum;
+  float* part_out;      // [num_seqs, num_heads, num_parts, head_dim]
+  cudaStream_t stream;
+};
+cf_status launch_block_scaled_attention(const BlockScaledLaunch& l);
+cf_status block_scaled_read_errors(uint32_t* bits, bool clear);
+
 }  // namespace cfb

@@ -34,6 +34,14 @@ __all__ = [
     "paged_attention_fp8_v1",
     "paged_attention_fp8_v2",
     "reshape_and_cache_fp8",
+    "rope_table",
+    "qk_norm_rope",
+    "rope_and_cache",
+    "rope_and_cache_fp8",
+    "rope_and_cache_fp8_block",
+    "reshape_and_cache_fp8_block",
+    "paged_attention_fp8_block_v1",
+    "paged_attention_fp8_block_workspace_size",
     "build_decode_inputs",
     "v2_num_partitions",
     "reshape_and_cache",
@@ -321,6 +329,216 @@ def reshape_and_cache_fp8(key, value, key_cache, value_cache, slot_mapping, k_sc
                                        num_blocks, dtype_code(key.dtype), float(k_scale), float(v_scale),
                                        _stream(key_cache)),
           "cf_reshape_and_cache_fp8")
+
+
+def _bad(what: str) -> CacheFlowError:
+    return CacheFlowError(_lib.CF_ERR_INVALID_ARGUMENT, what)
+
+
+def _on_device(call, t: torch.Tensor, what: str) -> None:
+    """Runs call(stream) on t's device and its current stream; raises on a status."""
+    if t.device.index == torch.cuda.current_device():
+        check(call(_stream(t)), what)
+    else:
+        with torch.cuda.device(t.device):
+            check(call(_stream(t)), what)
+
+
+def rope_table(max_positions: int, rotary_dim: int, base: float = 10000.0, device="cuda") -> torch.Tensor:
+    """cos_sin for the rotation: float32 [max_positions, rotary_dim], row p the cosines, then the sines, of
+    p * base^(-2i / rotary_dim) for i < rotary_dim / 2, the angles made in float64 (a float32 angle of a far
+    position is off by as much as 2^-8).  Scaled or otherwise changed frequencies: any table of that layout."""
+    if max_positions <= 0 or rotary_dim < 2 or rotary_dim % 2:
+        raise _bad("rope_table: max_positions > 0, rotary_dim even")
+    i = torch.arange(rotary_dim // 2, dtype=torch.float64, device=device)
+    a = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] * base ** (-2.0 * i / rotary_dim)
+    return torch.cat([a.cos(), a.sin()], dim=1).to(torch.float32)
+
+
+def _rope_params(q_out, query, key, positions, cos_sin, q_weight, k_weight, eps, interleaved, value=None,
+                 k_out=None):
+    if query.dim() != 3 or key.dim() != 3:
+        raise _bad("query/key must be [num_tokens, heads, head_dim]")
+    T, H, D = query.shape
+    Hkv = key.shape[1]
+    dt, dev = query.dtype, query.device
+    if not query.is_cuda:
+        raise _bad("query must be a CUDA tensor")
+    p = _lib.RopeParams()
+    for name, t, shape in (("query", query, (T, H, D)), ("key", key, (T, Hkv, D)), ("value", value, (T, Hkv, D)),
+                           ("query_out", q_out, (T, H, D)), ("key_out", k_out, (T, Hkv, D))):
+        if t is None:
+            continue
+        if tuple(t.shape) != shape or t.dtype != dt or t.device != dev:
+            raise _bad(f"{name} must be {dt} of shape {shape} on {dev}")
+        st = t.stride()
+        if st[2] != 1 and D > 1:
+            raise _bad(f"{name}: the last dimension must be contiguous")
+        setattr(p, name, t.data_ptr())
+        getattr(p, name + "_stride")[:] = st[:2]
+    if positions.dtype != torch.int32 or positions.shape != (T,) or not positions.is_contiguous() \
+            or positions.device != dev:
+        raise _bad(f"positions must be contiguous int32 of shape ({T},) on {dev}")
+    if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous() or cos_sin.device != dev:
+        raise _bad(f"cos_sin must be contiguous float32 [max_positions, rotary_dim] on {dev}")
+    p.positions, p.cos_sin = positions.data_ptr(), cos_sin.data_ptr()
+    p.dtype = p.weight_dtype = dtype_code(dt)
+    given = [w for w in (q_weight, k_weight) if w is not None]
+    for w in given:
+        if w.shape != (D,) or not w.is_contiguous() or w.device != dev or w.dtype not in (dt, torch.float32) \
+                or w.dtype != given[0].dtype:
+            raise _bad(f"norm weights must be contiguous ({D},) on {dev}, both float32 or both {dt}")
+    if given:
+        p.weight_dtype = dtype_code(given[0].dtype)
+        p.query_weight, p.key_weight = _ptr(q_weight), _ptr(k_weight)
+    p.num_tokens, p.num_heads, p.num_kv_heads, p.head_dim = T, H, Hkv, D
+    p.max_positions, p.rotary_dim = cos_sin.shape
+    p.eps = float(eps)
+    p.interleaved = 1 if interleaved else 0
+    return p
+
+
+def qk_norm_rope(q_out, k_out, query, key, positions, cos_sin, q_weight=None, k_weight=None, eps=1e-6,
+                 interleaved=False) -> None:
+    """Per-head RMS norms of Q and K (with a weight) and the position rotation, one launch.
+
+    query/q_out [T, H, D], key/k_out [T, Hkv, D] (f32, f16 or bf16; token and
+    head strides free, so slices of one fused projection do, and an output may
+    be its input); positions int32 [T], a negative one leaves the token's rows
+    unwritten; cos_sin as rope_table() gives it, its width the rotated columns;
+    weights [D] in float32 or the rows' type.  interleaved pairs columns (2i,
+    2i + 1) instead of (i, i + rotary_dim / 2).
+    """
+    lib = _lib.load()
+    if k_out is None:
+        raise _bad("k_out is needed")
+    p = _rope_params(q_out, query, key, positions, cos_sin, q_weight, k_weight, eps, interleaved, k_out=k_out)
+    _on_device(lambda st: lib.cf_qk_norm_rope(ctypes.byref(p), st), query, "cf_qk_norm_rope")
+
+
+def _check_caches(key_cache, value_cache, key, dt, slot_mapping):
+    if key_cache.dim() != 4 or key_cache.shape != value_cache.shape or key_cache.shape[1] != key.shape[1] \
+            or key_cache.shape[3] != key.shape[2]:
+        raise _bad("caches must be [num_blocks, num_kv_heads, block_size, head_dim] with key's heads and head_dim")
+    for t in (key_cache, value_cache):
+        if t.dtype != dt or not t.is_contiguous() or t.device != key.device:
+            raise _bad(f"caches must be contiguous {dt} on {key.device}")
+    if slot_mapping.dtype != torch.int32 or slot_mapping.shape != (key.shape[0],) \
+            or not slot_mapping.is_contiguous() or slot_mapping.device != key.device:
+        raise _bad(f"slot_mapping must be contiguous int32 of shape ({key.shape[0]},) on {key.device}")
+
+
+def _check_scales(k_scales, v_scales, key_cache):
+    for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
+        if t.dtype != torch.float32 or t.shape != key_cache.shape[:2] or not t.is_contiguous() \
+                or t.device != key_cache.device:
+            raise _bad(f"{name} must be contiguous float32 {tuple(key_cache.shape[:2])} on {key_cache.device}")
+
+
+def rope_and_cache(q_out, query, key, value, key_cache, value_cache, slot_mapping, positions, cos_sin, q_weight=None,
+                   k_weight=None, eps=1e-6, interleaved=False) -> None:
+    """qk_norm_rope with the append in it, one launch: Q goes to q_out, K (normed, rotated) and V to their slots
+    of caches of their own dtype, as reshape_and_cache writes them (a negative slot appends nothing)."""
+    lib = _lib.load()
+    p = _rope_params(q_out, query, key, positions, cos_sin, q_weight, k_weight, eps, interleaved, value=value)
+    _check_caches(key_cache, value_cache, key, query.dtype, slot_mapping)
+    _on_device(lambda st: lib.cf_rope_and_cache(ctypes.byref(p), _ptr(key_cache), _ptr(value_cache),
+                                                _ptr(slot_mapping), key_cache.shape[2], key_cache.shape[0], st),
+               query, "cf_rope_and_cache")
+
+
+def rope_and_cache_fp8(q_out, query, key, value, key_cache, value_cache, slot_mapping, positions, cos_sin, k_scale,
+                       v_scale, q_weight=None, k_weight=None, eps=1e-6, interleaved=False) -> None:
+    """rope_and_cache into float8_e4m3fn caches with one scale each: cache = e4m3(x / scale), from the f32 rows."""
+    lib = _lib.load()
+    p = _rope_params(q_out, query, key, positions, cos_sin, q_weight, k_weight, eps, interleaved, value=value)
+    _check_caches(key_cache, value_cache, key, torch.float8_e4m3fn, slot_mapping)
+    _on_device(lambda st: lib.cf_rope_and_cache_fp8(ctypes.byref(p), _ptr(key_cache), _ptr(value_cache),
+                                                    _ptr(slot_mapping), key_cache.shape[2], key_cache.shape[0],
+                                                    float(k_scale), float(v_scale), st),
+               query, "cf_rope_and_cache_fp8")
+
+
+def rope_and_cache_fp8_block(q_out, query, key, value, key_cache, value_cache, k_scales, v_scales, slot_mapping,
+                             positions, cos_sin, q_weight=None, k_weight=None, eps=1e-6, interleaved=False) -> None:
+    """rope_and_cache into float8_e4m3fn caches with a scale for each block and KV head (rules as
+    reshape_and_cache_fp8_block, from the f32 rows)."""
+    lib = _lib.load()
+    p = _rope_params(q_out, query, key, positions, cos_sin, q_weight, k_weight, eps, interleaved, value=value)
+    _check_caches(key_cache, value_cache, key, torch.float8_e4m3fn, slot_mapping)
+    _check_scales(k_scales, v_scales, key_cache)
+    _on_device(lambda st: lib.cf_rope_and_cache_fp8_block(ctypes.byref(p), _ptr(key_cache), _ptr(value_cache),
+                                                          _ptr(k_scales), _ptr(v_scales), _ptr(slot_mapping),
+                                                          key_cache.shape[2], key_cache.shape[0], st),
+               query, "cf_rope_and_cache_fp8_block")
+
+
+def reshape_and_cache_fp8_block(key, value, key_cache, value_cache, k_scales, v_scales, slot_mapping) -> None:
+    """reshape_and_cache into float8_e4m3fn caches with a scale for each block and KV head.
+
+    k_scales / v_scales float32 [num_blocks, num_kv_heads], 0 in a new pool: a
+    block's scale is the smallest power of two that its rows need (max |x| <=
+    448 scale); a call that writes the block's offset 0 starts it over, any
+    other one raises the scale where its rows need it and stores the rows that
+    are there anew.  Scales move with their blocks: copy_blocks and the other
+    block operators take scales.view(num_blocks, num_kv_heads, 1, 1).
+    """
+    lib = _lib.load()
+    if key.dim() != 3 or key.shape != value.shape or key.dtype != value.dtype or key.device != value.device \
+            or not key.is_cuda:
+        raise _bad("key/value must be CUDA tensors [num_tokens, num_kv_heads, head_dim] of one dtype")
+    T, Hkv, D = key.shape
+    dense = key.is_contiguous() and value.is_contiguous()
+    _check_caches(key_cache, value_cache, key, torch.float8_e4m3fn, slot_mapping)
+    _check_scales(k_scales, v_scales, key_cache)
+    if not dense:  # strided rows (slices of a fused projection)
+        key, value = key.contiguous(), value.contiguous()
+    _on_device(lambda st: lib.cf_reshape_and_cache_fp8_block(
+        _ptr(key), _ptr(value), _ptr(key_cache), _ptr(value_cache), _ptr(k_scales), _ptr(v_scales),
+        _ptr(slot_mapping), T, Hkv, D, key_cache.shape[2], key_cache.shape[0], dtype_code(key.dtype), st),
+        key, "cf_reshape_and_cache_fp8_block")
+
+
+def paged_attention_fp8_block_workspace_size(query, key_cache, block_tables, max_context_len) -> int:
+    """Bytes of optional workspace that lets paged_attention_fp8_block_v1 split long contexts."""
+    lib = _lib.load()
+    p = AttentionParams()
+    p.num_seqs = query.shape[0]
+    p.num_heads = query.shape[1]
+    p.num_blocks, p.num_kv_heads, p.block_size, p.head_dim = key_cache.shape
+    p.max_context_len = int(max_context_len)
+    p.max_blocks_per_seq = block_tables.shape[1]
+    p.dtype = dtype_code(query.dtype)
+    return int(lib.cf_paged_attention_fp8_block_workspace_size(ctypes.byref(p)))
+
+
+def paged_attention_fp8_block_v1(out, query, key_cache, value_cache, k_scales, v_scales, block_tables, context_lens,
+                                 scale=None, max_context_len=None,
+                                 workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Decode attention over float8_e4m3fn caches whose blocks have a scale for each KV head (K = k_scales[block,
+    head] * stored, V alike; as reshape_and_cache_fp8_block fills them); query and output f16 or bf16, head_dim 128
+    or 256.  The workspace (paged_attention_fp8_block_workspace_size bytes) lets long contexts split."""
+    lib = _lib.load()
+    if scale is None:
+        scale = 1.0 / math.sqrt(query.shape[-1])
+    if max_context_len is None:
+        max_context_len = int(context_lens.max().item()) if context_lens.numel() else 0
+    p = _attention_params(out, query, key_cache, value_cache, block_tables, context_lens, scale,
+                          max_context_len, fp8=True)
+    S, H, D = query.shape
+    if out.shape != query.shape or value_cache.shape != key_cache.shape or key_cache.shape[3] != D \
+            or context_lens.shape != (S,) or block_tables.dim() != 2 or block_tables.shape[0] != S:
+        raise _bad("paged_attention_fp8_block_v1: shapes of query, out, caches, block_tables and context_lens differ")
+    for t in (out, key_cache, value_cache, block_tables, context_lens):
+        if t.device != query.device:
+            raise _bad(f"paged_attention_fp8_block_v1: every tensor must be on {query.device}")
+    _check_scales(k_scales, v_scales, key_cache)
+    ws = _ptr(workspace)
+    ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    _on_device(lambda st: lib.cf_paged_attention_fp8_block_v1(ctypes.byref(p), _ptr(k_scales), _ptr(v_scales), ws,
+                                                              ws_bytes, st),
+               query, "cf_paged_attention_fp8_block_v1")
+    return out
 
 
 def build_decode_inputs(positions, block_offsets, block_ids, max_blocks_per_seq, block_size=16,

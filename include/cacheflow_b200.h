@@ -60,6 +60,7 @@ typedef enum cf_dtype {
 #define CF_DEVERR_SLOT 0x2u        /* slot_mapping entry outside the pool              */
 #define CF_DEVERR_CONTEXT_LEN 0x4u /* context length < 0 or > max_blocks_per_seq*bs   */
 #define CF_DEVERR_TIMEOUT 0x8u     /* a bounded pipeline wait gave up (kernel returned) */
+#define CF_DEVERR_POSITION 0x10u   /* token position outside the rotation's angle table */
 
 /* Parameters of one paged decode-attention call.  Same fields and meaning as
  * cacheflow::cuda::PagedAttentionParams (paged_attention.cuh:25-40) plus
@@ -291,6 +292,124 @@ CF_API cf_status cf_reshape_and_cache(const void* key, const void* value,
                                int32_t num_kv_heads, int32_t head_dim,
                                int32_t block_size, int64_t num_blocks,
                                int32_t dtype, void* stream);
+
+/* Parameters of the query/key pass between a layer's projection and its
+ * attention: per-head RMS norms and the position rotation, computed in f32
+ * and rounded once.  For each token t with position p = positions[t] and each
+ * head row x of head_dim elements:
+ *   norm     x * rsqrt(mean(x^2) + eps) * weight, where the weight is given
+ *   rotation columns below rotary_dim in pairs (a, b) = (i, i + rotary_dim/2),
+ *            or (2i, 2i + 1) with `interleaved`:
+ *              a cos_i - b sin_i,  b cos_i + a sin_i
+ *            cos_sin[p] holds rotary_dim/2 cosines, then as many sines; the
+ *            columns from rotary_dim on pass.
+ * A token with a negative position is padding: none of its rows are written,
+ * to the outputs or to a cache.  A position of max_positions or more is
+ * recorded (CF_DEVERR_POSITION) and treated the same way.
+ * Rows may be strided (slices of one fused projection buffer): strides are in
+ * elements, {token, head}, and a row's head_dim elements are contiguous.  An
+ * output may be its input itself (same pointer and strides); other overlaps
+ * are not allowed.  Pointers and strides of 16 bytes run widest. */
+typedef struct cf_rope_params {
+  const void* query;         /* [num_tokens, num_heads, head_dim]             */
+  const void* key;           /* [num_tokens, num_kv_heads, head_dim]          */
+  const void* value;         /* as key; cache forms only                      */
+  void* query_out;           /* as query                                      */
+  void* key_out;             /* as key; cf_qk_norm_rope only                  */
+  const int32_t* positions;  /* [num_tokens]                                  */
+  const float* cos_sin;      /* [max_positions, rotary_dim]                   */
+  const void* query_weight;  /* [head_dim] or NULL: no norm                   */
+  const void* key_weight;    /* [head_dim] or NULL                            */
+  int64_t query_stride[2];
+  int64_t key_stride[2];
+  int64_t value_stride[2];
+  int64_t query_out_stride[2];
+  int64_t key_out_stride[2];
+  int32_t num_tokens;
+  int32_t num_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;          /* even, up to 256                               */
+  int32_t rotary_dim;        /* even, 2..head_dim                             */
+  int32_t max_positions;
+  float eps;                 /* > 0 where a weight is given                   */
+  int32_t interleaved;       /* 0 or 1                                        */
+  int32_t dtype;             /* CF_F32, CF_F16 or CF_BF16                     */
+  int32_t weight_dtype;      /* CF_F32 or dtype                               */
+} cf_rope_params;
+
+/* Norms and rotation of Q and K into query_out and key_out, one launch.  No
+ * CacheFlow counterpart (its forward pass is the abstract ForwardFn of
+ * batch_decode.h:34-42). */
+CF_API cf_status cf_qk_norm_rope(const cf_rope_params* params, void* stream);
+
+/* The same pass with the append in it: query_out as cf_qk_norm_rope gives it,
+ * and K (normed, rotated) and V of each token written to its cache slot, as
+ * cf_reshape_and_cache would write them (slots, padding and range checks
+ * alike); caches of params->dtype, V's rows bit for bit. */
+CF_API cf_status cf_rope_and_cache(const cf_rope_params* params, void* key_cache, void* value_cache,
+                                   const int32_t* slot_mapping, int32_t block_size,
+                                   int64_t num_blocks, void* stream);
+
+/* cf_rope_and_cache into e4m3 caches with one scale each, quantized from the
+ * f32 rows as cf_reshape_and_cache_fp8 quantizes (head_dim a multiple of 16,
+ * caches 16-byte aligned). */
+CF_API cf_status cf_rope_and_cache_fp8(const cf_rope_params* params, void* key_cache,
+                                       void* value_cache, const int32_t* slot_mapping,
+                                       int32_t block_size, int64_t num_blocks, float k_scale,
+                                       float v_scale, void* stream);
+
+/* Append into e4m3 caches with a scale for each block and KV head: the stored
+ * bytes times k_scales[block, head] / v_scales[block, head] are K and V.  For
+ * the rows that the call appends to a block, head by head and K and V apart:
+ *   need = the smallest power of two s with max |x| <= 448 s (finite x; 0 if
+ *          all are 0)
+ *   a call that writes the block's offset 0 starts the block over: its scale
+ *   becomes need, its other rows keep their (now meaningless) bytes;
+ *   otherwise its scale becomes max(old scale, need), and where that grew, the
+ *   other rows are stored anew as e4m3(byte * old / new).
+ * Bytes are e4m3(x / scale), to nearest even, saturating at +-448.  With
+ * power-of-two scales the division is exact and storing rows anew loses
+ * nothing but what falls under e4m3's smallest normal.  A new pool's scales
+ * start at 0.  Rows of a block may come in any order and place of the call;
+ * of two tokens with one slot the later is stored (calls of more than 16384
+ * tokens count as consecutive calls of 16384).  The scale arrays move with
+ * their blocks: cf_copy_blocks and the other block operators take them as
+ * caches of block_size 1, head_dim 1, CF_F32.
+ * key, value [num_tokens, num_kv_heads, head_dim], contiguous, of `dtype`
+ * (CF_F32, CF_F16 or CF_BF16); head_dim a multiple of 16 up to 256;
+ * block_size 16; num_blocks > 0; caches 16-byte aligned. */
+CF_API cf_status cf_reshape_and_cache_fp8_block(const void* key, const void* value,
+                                                void* key_cache, void* value_cache,
+                                                float* k_scales, float* v_scales,
+                                                const int32_t* slot_mapping, int32_t num_tokens,
+                                                int32_t num_kv_heads, int32_t head_dim,
+                                                int32_t block_size, int64_t num_blocks,
+                                                int32_t dtype, void* stream);
+
+/* cf_rope_and_cache into e4m3 caches with a scale for each block and head
+ * (rules as cf_reshape_and_cache_fp8_block, from the f32 rows). */
+CF_API cf_status cf_rope_and_cache_fp8_block(const cf_rope_params* params, void* key_cache,
+                                             void* value_cache, float* k_scales, float* v_scales,
+                                             const int32_t* slot_mapping, int32_t block_size,
+                                             int64_t num_blocks, void* stream);
+
+/* Decode attention over e4m3 caches with a scale for each block and KV head:
+ * K = k_scales[block, head] * stored, V = v_scales[block, head] * stored
+ * (f32, finite, >= 0; [num_blocks, num_kv_heads]).  params->dtype is the type
+ * of the query and the output (CF_F16 or CF_BF16); head_dim 128 or 256;
+ * num_blocks > 0.  A row with context 0 gives zeros.  The workspace is
+ * optional: with at least cf_paged_attention_fp8_block_workspace_size() bytes
+ * (16-byte aligned) long contexts are split across CTAs and merged by a
+ * second kernel.  Two calls that may overlap need workspaces of their own. */
+CF_API cf_status cf_paged_attention_fp8_block_v1(const cf_paged_attention_params* params,
+                                                 const float* k_scales, const float* v_scales,
+                                                 void* workspace, size_t workspace_bytes,
+                                                 void* stream);
+
+/* Bytes of workspace the split of cf_paged_attention_fp8_block_v1 uses for
+ * these params or for the same sizes with any shorter max_context_len; 0: it
+ * never splits. */
+CF_API size_t cf_paged_attention_fp8_block_workspace_size(const cf_paged_attention_params* params);
 
 /* Copy whole K and V blocks within one cache (copy-on-write forks):
  * for each pair i, block block_mapping[2i+1] := block block_mapping[2i].
