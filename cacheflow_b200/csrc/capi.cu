@@ -255,7 +255,7 @@ size_t block_split(const cf_paged_attention_params* p, int32_t* parts_out, int32
   constexpr int64_t kTargetCtas = 4 * 148;
   const int64_t pairs = (int64_t)p->num_seqs * p->num_kv_heads;
   int32_t split = 2048;
-  while (split > 256 && pairs * ((p->max_context_len + split - 1) / split) < kTargetCtas) split /= 2;
+  while (split > 128 && pairs * ((p->max_context_len + split - 1) / split) < kTargetCtas) split /= 2;
   if (p->max_context_len <= split) return 0;
   const int64_t parts = ((int64_t)p->max_context_len + split - 1) / split;
   if (parts_out) *parts_out = (int32_t)parts;
@@ -574,7 +574,9 @@ cf_status cf_paged_attention_fp8_block_v1(const cf_paged_attention_params* p, co
   if (st != CF_OK) return st;
   if ((st = check_fp8(p, 1.f, 1.f)) != CF_OK || p->num_seqs == 0) return st;
   if (!k_scales || !v_scales || p->num_blocks <= 0) return CF_ERR_INVALID_ARGUMENT;
-  if (p->num_blocks * (int64_t)p->num_kv_heads * p->block_size > INT32_MAX) return CF_ERR_UNSUPPORTED;
+  // TMA rows and token counts are int32
+  if (p->num_blocks > INT32_MAX / p->block_size / p->num_kv_heads || p->max_blocks_per_seq > (INT32_MAX - 128) / 16)
+    return CF_ERR_UNSUPPORTED;
   BlockScaledLaunch l{p, k_scales, v_scales, 0, 1, nullptr, nullptr, nullptr, (cudaStream_t)stream};
   int32_t parts = 1, tokens = 0;
   const size_t need = block_split(p, &parts, &tokens);

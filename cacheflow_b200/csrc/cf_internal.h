@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/cacheflow_b200.h"
 
 namespace cfb {
@@ -52,6 +54,9 @@ bool attention_fp8_supported(int32_t head_dim, int32_t block_size, int32_t dtype
 // swizzle; false if it cannot be encoded.
 bool kv_tensor_map(CUtensorMap* map, const void* base, int64_t rows, int D, int32_t dtype);
 cf_status attention_read_errors(uint32_t* bits, bool clear);
+// Test hooks of the decode kernels' bounded waits (cf_testing_set_pipeline_faults).
+extern std::atomic<int64_t> g_test_wait_limit_ns;
+extern std::atomic<int32_t> g_test_unarm_first_stage;
 
 // ---- chunked-prefill attention (prefill_attention.cu) ------------------------
 bool prefill_supported(int32_t head_dim, int32_t block_size, int32_t dtype, int32_t group);
