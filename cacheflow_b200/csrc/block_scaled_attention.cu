@@ -10,6 +10,7 @@
 // 2^(x_t) / vs[b_t].  A block whose vs is 0 adds to L alone.
 #include <cmath>
 #include <mutex>
+#include <type_traits>
 
 #include "cf_device.cuh"
 #include "cf_internal.h"
@@ -89,18 +90,28 @@ constexpr int kProducerWarp = 4;
 constexpr int kMmaWarp = 5;
 constexpr float kPScale = 256.f;
 
-template <int D, int HG>
+// e4m3 terms of a query element and of a weight: two hold a bf16's 8
+// significant bits, three an f16's 11.
+template <typename T>
+constexpr int kTerms = std::is_same<T, __half>::value ? 3 : 2;
+
+template <typename T, int D, int HG>
 struct Layout {
-  static constexpr int kN = (3 * HG + 15) / 16 * 16;  // MMA columns
+  static constexpr int kN = (kTerms<T> * HG + 15) / 16 * 16;  // MMA columns
   static constexpr int kBoxes = D / 128;
   static constexpr int kHalf = kBoxes * kBox;         // a tile's K or V
-  static constexpr int kStage = 2 * kHalf;
-  static constexpr int kStages = 3;
-  static constexpr int kQOff = kStages * kStage;      // Q: kBoxes x [kN rows x 128 B]
+  // K and V have rings of their own: a K stage is free once its QK is done,
+  // a V stage an exchange of maxima and a PV later.
+  static constexpr bool kThree = D == 128 && kN == 16;  // three CTAs per SM
+  static constexpr int kStages = kThree ? 2 : 3;
+  static constexpr int kVOff = kStages * kHalf;
+  static constexpr int kQOff = 2 * kStages * kHalf;   // Q: kBoxes x [kN rows x 128 B]
   static constexpr int kQBox = kN * 128;
-  static constexpr int kPOff = kQOff + kBoxes * kQBox;  // P: 2 x [kN rows x 128 B]
-  static constexpr int kBarOff = kPOff + 2 * kQBox;
-  static constexpr int kNumBars = 2 * kStages + 4 * 2 + 1;  // full, empty; s_full, p_full, o_full, top; fin
+  static constexpr int kPOff = kQOff + kBoxes * kQBox;  // P: 2 x [kN/16 planes x 128 tokens x 16 B]
+  static constexpr int kPBytes = kN * 128;
+  static constexpr int kBarOff = kPOff + 2 * kPBytes;
+  // full, empty of K and of V; s_full, p_full, o_full, top by tile parity; fin
+  static constexpr int kNumBars = 4 * kStages + 4 * 2 + 1;
   static constexpr int kMaxOff = kBarOff + (kNumBars * 8 + 15) / 16 * 16;  // [2][4][HG] f32
   static constexpr int kMaxHeads = (HG + 3) / 4 * 4;
   static constexpr int kSumOff = kMaxOff + 2 * 4 * kMaxHeads * 4;          // [4][HG] f32
@@ -109,6 +120,7 @@ struct Layout {
   static constexpr int kTmemOff = kOkOff + 16;
   static constexpr int kBytes = kTmemOff + 16;
   static constexpr int kAlloc = kBytes + 1024;
+  static constexpr int kMinCtas = kThree ? 3 : (D == 128 ? 2 : 1);
   static constexpr int kOCol = 2 * kN;                 // O after the two S buffers
   static constexpr int kCols = 2 * kN + 2 * kBoxes * kN;
   static constexpr uint32_t kTmemCols = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
@@ -116,9 +128,15 @@ struct Layout {
 };
 
 // Instruction descriptor of kind::f8f6f4: f32 accumulation, A and B e4m3,
-// A K-major or MN-major, B K-major.
-__host__ __device__ constexpr uint32_t idesc_f8(uint32_t a_mn_major, uint32_t n) {
-  return (1u << 4) | (a_mn_major << 15) | ((n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+// A and B K-major (0) or MN-major (1).
+__host__ __device__ constexpr uint32_t idesc_f8(uint32_t mn_major, uint32_t n) {
+  return (1u << 4) | (mn_major << 15) | (mn_major << 16) | ((n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+}
+
+// Matrix descriptor without a swizzle (version 1, layout type 0).
+__device__ __forceinline__ uint64_t smem_desc_plain(uint32_t saddr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
+  return (uint64_t)((saddr >> 4) & 0x3fffu) | ((uint64_t)((lbo_bytes >> 4) & 0x3fffu) << 16) |
+         ((uint64_t)((sbo_bytes >> 4) & 0x3fffu) << 32) | (1ull << 46);
 }
 
 __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -142,36 +160,47 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// Max over the warp (order-preserving map of f32 to signed integers).
+// Max over the warp; a NaN takes no part.
 __device__ __forceinline__ float warp_max(float x) {
-  int i = __float_as_int(x);
-  i = i >= 0 ? i : i ^ 0x7fffffff;
-  i = __reduce_max_sync(0xffffffffu, i);
-  return __int_as_float(i >= 0 ? i : i ^ 0x7fffffff);
+  float m;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(x));
+  return m;
 }
 
-__device__ __forceinline__ float2 e4m3x2_to_f2(uint16_t c) {
-  const uint32_t h = e4m3x2_to_h2(c);
-  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+__device__ __forceinline__ uint16_t h2_to_e4m3x2(__half2 h) {
+  return (uint16_t)__nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(h), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ __half2 e4m3x2_to_half2(uint16_t c) {
+  return __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)c, __NV_E4M3));
 }
 
-// x, y -> three e4m3 terms each (x in the low bytes).
-__device__ __forceinline__ void three_terms(float x, float y, uint16_t (&t)[3]) {
-  t[0] = f2_to_e4m3x2(x, y);
-  float2 b = e4m3x2_to_f2(t[0]);
-  x = (x - b.x) * 16.f;
-  y = (y - b.y) * 16.f;
-  t[1] = f2_to_e4m3x2(x, y);
-  b = e4m3x2_to_f2(t[1]);
-  t[2] = f2_to_e4m3x2((x - b.x) * 16.f, (y - b.y) * 16.f);
+// Two f16 values -> kT e4m3 terms each: x = t1 + t2/16 + t3/256, every term
+// the rounding of 16 times what the ones before it leave (exact in f16).
+template <int kT>
+__device__ __forceinline__ void split_terms(__half2 x, uint16_t (&t)[kT]) {
+  const __half2 sixteen = __float2half2_rn(16.f);
+#pragma unroll
+  for (int i = 0; i < kT; ++i) {
+    t[i] = h2_to_e4m3x2(x);
+    if (i + 1 < kT) x = __hmul2(__hsub2(x, e4m3x2_to_half2(t[i])), sixteen);
+  }
+}
+
+// The sum of a head's terms: columns h, HG + h, ... of v.
+template <int kT, int HG>
+__device__ __forceinline__ float join_terms(const float* v, int h) {
+  float r = v[(kT - 1) * HG + h];
+#pragma unroll
+  for (int i = kT - 2; i >= 0; --i) r = fmaf(r, 0.0625f, v[i * HG + h]);
+  return r;
 }
 
 template <typename T, int D, int HG>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
     block_attention_kernel(const Args a, const __grid_constant__ CUtensorMap tmk,
                            const __grid_constant__ CUtensorMap tmv) {
-  using L = Layout<D, HG>;
-  constexpr int N = L::kN, S = L::kStages;
+  using L = Layout<T, D, HG>;
+  constexpr int N = L::kN, S = L::kStages, kT = kTerms<T>;
   const int part = blockIdx.x, seq = blockIdx.z;
   const int kvh = blockIdx.y / a.head_chunks, chunk = blockIdx.y - kvh * a.head_chunks;
   const int head0 = kvh * a.group + chunk * HG;
@@ -192,9 +221,11 @@ __global__ void __launch_bounds__(kThreads)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
-  uint64_t* full = bars;
-  uint64_t* empty = bars + S;
-  uint64_t* s_full = bars + 2 * S;  // [2], by tile parity, as the ones below
+  uint64_t* k_full = bars;
+  uint64_t* k_empty = bars + S;
+  uint64_t* v_full = bars + 2 * S;
+  uint64_t* v_empty = bars + 3 * S;
+  uint64_t* s_full = bars + 4 * S;  // [2], by tile parity, as the ones below
   uint64_t* p_full = s_full + 2;
   uint64_t* o_full = p_full + 2;
   uint64_t* top = o_full + 2;
@@ -207,38 +238,44 @@ __global__ void __launch_bounds__(kThreads)
 
   int ids = 0, ids_next = 0;  // producer: block ids of this and the next 32 blocks
   auto load_ids = [&](int b) { return b + lane < nblk ? table[b + lane] : 0; };
-  auto produce = [&](int j) {
-    const int s = j % S;
+  int id = 0;
+  bool valid_id = false;
+  auto produce_k = [&](int j) {  // takes the tile's ids, then copies K
     const int b0 = j * kTileBlocks;
     if ((b0 & 31) == 0) {
       ids = b0 == 0 ? load_ids(0) : ids_next;
       ids_next = load_ids(b0 + 32);
     }
-    const int id = __shfl_sync(0xffffffffu, ids, (b0 & 31) + (lane & 7));
+    id = __shfl_sync(0xffffffffu, ids, (b0 & 31) + (lane & 7));
     const bool want = lane < kTileBlocks && b0 + lane < nblk;
-    const bool valid = want && id >= 0 && (int64_t)id < a.num_blocks;
-    if (want && !valid) block_attn_error(CF_DEVERR_BLOCK_ID);
-    const uint32_t mask = __ballot_sync(0xffffffffu, valid);
+    valid_id = want && id >= 0 && (int64_t)id < a.num_blocks;
+    if (want && !valid_id) block_attn_error(CF_DEVERR_BLOCK_ID);
+  };
+  // Copies the tile's K or V: lane k block k, onto the stage's barrier.
+  auto copy = [&](int j, const CUtensorMap* map, uint64_t* full, uint8_t* ring) {
     if (a.unarm_first_stage && j == 0) return;  // test hook: the stage never completes
-    const uint32_t bar = smem_addr(&full[s]);
+    const uint32_t bar = smem_addr(&full[j % S]);
+    const uint32_t mask = __ballot_sync(0xffffffffu, valid_id);
     if (lane == 0) {
       fence_proxy_async_smem();
       if (mask == 0)
         mbar_arrive(bar);
       else
-        mbar_arrive_expect_tx(bar, (uint32_t)__popc(mask) * 2 * kBlk * D);
+        mbar_arrive_expect_tx(bar, (uint32_t)__popc(mask) * kBlk * D);
     }
     __syncwarp();
-    if (valid) {  // lane k copies block k
+    if (valid_id) {
       const int32_t row = (int32_t)(((int64_t)id * a.num_kv_heads + kvh) * kBlk);
-      uint8_t* k = smem + s * L::kStage + lane * (kBlk * 128);
+      uint8_t* dst = ring + (j % S) * L::kHalf + lane * (kBlk * 128);
 #pragma unroll
-      for (int b = 0; b < L::kBoxes; ++b) {
-        tma_load_2d(smem_addr(k + b * kBox), &tmk, b * 128, row, bar);
-        tma_load_2d(smem_addr(k + L::kHalf + b * kBox), &tmv, b * 128, row, bar);
-      }
+      for (int b = 0; b < L::kBoxes; ++b) tma_load_2d(smem_addr(dst + b * kBox), map, b * 128, row, bar);
     }
     __syncwarp();
+  };
+  auto produce = [&](int j) {
+    produce_k(j);
+    copy(j, &tmk, k_full, smem);
+    copy(j, &tmv, v_full, smem + L::kVOff);
   };
 
   // Set-up: the producer starts copying as soon as the barriers are there;
@@ -247,8 +284,10 @@ __global__ void __launch_bounds__(kThreads)
   if (warp == kProducerWarp) {
     if (lane == 0) {
       for (int s = 0; s < S; ++s) {
-        mbar_init(smem_addr(&full[s]), 1);
-        mbar_init(smem_addr(&empty[s]), 1);
+        mbar_init(smem_addr(&k_full[s]), 1);
+        mbar_init(smem_addr(&k_empty[s]), 1);
+        mbar_init(smem_addr(&v_full[s]), 1);
+        mbar_init(smem_addr(&v_empty[s]), 1);
       }
       for (int i = 0; i < 2; ++i) {
         mbar_init(smem_addr(&s_full[i]), 1);
@@ -265,12 +304,9 @@ __global__ void __launch_bounds__(kThreads)
     tmem_alloc(smem_addr(tmem_slot), L::kTmemCols);
     tmem_relinquish();
   } else {
-    // P's unused rows are zero for good
-    for (int i = threadIdx.x; i < 2 * N * 8; i += kTile)
-      reinterpret_cast<uint4*>(smem + L::kPOff)[i] = make_uint4(0, 0, 0, 0);
     constexpr int E = D / 32;
     for (int n = warp; n < N; n += 4) {  // rows past the terms
-      if (n >= 3 * HG)
+      if (n >= kT * HG)
         for (int b = 0; b < L::kBoxes; ++b)
           reinterpret_cast<uint32_t*>(smem + L::kQOff + b * L::kQBox + n * 128)[lane] = 0u;
     }
@@ -297,12 +333,12 @@ __global__ void __launch_bounds__(kThreads)
       const float inv = __uint_as_float((uint32_t)(254 - ex) << 23);
 #pragma unroll
       for (int e = 0; e < E; e += 4) {
-        uint16_t lo[3], hi[3];
-        three_terms(q[e] * inv, q[e + 1] * inv, lo);
-        three_terms(q[e + 2] * inv, q[e + 3] * inv, hi);
+        uint16_t lo[kT], hi[kT];
+        split_terms<kT>(__floats2half2_rn(q[e] * inv, q[e + 1] * inv), lo);
+        split_terms<kT>(__floats2half2_rn(q[e + 2] * inv, q[e + 3] * inv), hi);
         const int col = lane * E + e;  // byte of the row
 #pragma unroll
-        for (int t = 0; t < 3; ++t) {
+        for (int t = 0; t < kT; ++t) {
           const int n = t * HG + h;
           uint32_t w = (uint32_t)lo[t] | ((uint32_t)hi[t] << 16);
           if (bad) w = 0x7f7f7f7fu;  // a query that is not finite has no softmax: NaN
@@ -323,27 +359,39 @@ __global__ void __launch_bounds__(kThreads)
     bool ok = true;
     for (; produced < ntiles; ++produced) {
       const int s = produced % S;
-      if (!mbar_wait_bounded(smem_addr(&empty[s]), (uint32_t)(produced / S - 1) & 1u, a.wait_limit_ns)) ok = false;
+      const uint32_t parity = (uint32_t)(produced / S - 1) & 1u;
+      produce_k(produced);
+      ok = mbar_wait_bounded(smem_addr(&k_empty[s]), parity, a.wait_limit_ns);
       if (!__all_sync(0xffffffffu, ok)) break;
-      produce(produced);
+      copy(produced, &tmk, k_full, smem);
+      ok = mbar_wait_bounded(smem_addr(&v_empty[s]), parity, a.wait_limit_ns);
+      if (!__all_sync(0xffffffffu, ok)) {
+        if (lane == 0) mbar_wait_bounded(smem_addr(&k_full[s]), (uint32_t)(produced / S) & 1u, a.wait_limit_ns);
+        break;
+      }
+      copy(produced, &tmv, v_full, smem + L::kVOff);
     }
-    if (!ok && lane == 0) block_attn_error(CF_DEVERR_TIMEOUT);
+    if (!ok) block_attn_error(CF_DEVERR_TIMEOUT);
     // no copy may land after the CTA has left
     if (lane == 0)
-      for (int j = produced > S ? produced - S : 0; j < produced; ++j)
-        mbar_wait_bounded(smem_addr(&full[j % S]), (uint32_t)(j / S) & 1u, a.wait_limit_ns);
+      for (int j = produced > S ? produced - S : 0; j < produced; ++j) {
+        mbar_wait_bounded(smem_addr(&k_full[j % S]), (uint32_t)(j / S) & 1u, a.wait_limit_ns);
+        mbar_wait_bounded(smem_addr(&v_full[j % S]), (uint32_t)(j / S) & 1u, a.wait_limit_ns);
+      }
   } else if (warp == kMmaWarp) {
     if (lane == 0) {
       const uint64_t k_desc = smem_desc_sw128(smem_addr(smem), 16, 1024);
-      const uint64_t v_desc = smem_desc_sw128(smem_addr(smem + L::kHalf), 16, 1024);
+      const uint64_t v_desc = smem_desc_sw128(smem_addr(smem + L::kVOff), 16, 1024);
       const uint64_t q_desc = smem_desc_sw128(smem_addr(smem + L::kQOff), 16, 1024);
-      const uint64_t p_desc = smem_desc_sw128(smem_addr(smem + L::kPOff), 16, 1024);
+      // P: 8 tokens x 16 columns per 128 bytes, tokens onward, then planes
+      const uint64_t p_desc = smem_desc_plain(smem_addr(smem + L::kPOff), 128, kTile * 16);
       bool ok = true;
       auto issue_qk = [&](int j) {
-        ok = ok && mbar_wait_bounded(smem_addr(&full[j % S]), (uint32_t)(j / S) & 1u, a.wait_limit_ns);
+        const int s = j % S;
+        ok = ok && mbar_wait_bounded(smem_addr(&k_full[s]), (uint32_t)(j / S) & 1u, a.wait_limit_ns);
         if (!ok) return;
         tc_fence_after();
-        const uint64_t kd = k_desc + (uint64_t)(((j % S) * L::kStage) >> 4);
+        const uint64_t kd = k_desc + (uint64_t)((s * L::kHalf) >> 4);
 #pragma unroll
         for (int kk = 0; kk < D / 32; ++kk) {
           const uint64_t ad = kd + (uint64_t)(((kk >> 2) * kBox + (kk & 3) * 32) >> 4);
@@ -351,18 +399,23 @@ __global__ void __launch_bounds__(kThreads)
           mma_f8(tmem + (j & 1) * N, ad, bd, idesc_f8(0, N), kk > 0 ? 1u : 0u);
         }
         tc_commit(smem_addr(&s_full[j & 1]));
+        tc_commit(smem_addr(&k_empty[s]));
       };
       auto issue_pv = [&](int j) {
-        const uint64_t vd = v_desc + (uint64_t)(((j % S) * L::kStage) >> 4);
-        const uint64_t pd = p_desc + (uint64_t)(((j & 1) * L::kQBox) >> 4);
+        const int s = j % S;
+        ok = mbar_wait_bounded(smem_addr(&v_full[s]), (uint32_t)(j / S) & 1u, a.wait_limit_ns);
+        if (!ok) return;
+        tc_fence_after();
+        const uint64_t vd = v_desc + (uint64_t)((s * L::kHalf) >> 4);
+        const uint64_t pd = p_desc + (uint64_t)(((j & 1) * L::kPBytes) >> 4);
 #pragma unroll
         for (int b = 0; b < L::kBoxes; ++b)
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)  // 32 tokens each
             mma_f8(tmem + L::kOCol + ((j & 1) * L::kBoxes + b) * N, vd + (uint64_t)((b * kBox + kk * 4096) >> 4),
-                   pd + (uint64_t)((kk * 32) >> 4), idesc_f8(1, N), kk > 0 ? 1u : 0u);
+                   pd + (uint64_t)((kk * 512) >> 4), idesc_f8(1, N), kk > 0 ? 1u : 0u);
         tc_commit(smem_addr(&o_full[j & 1]));
-        tc_commit(smem_addr(&empty[j % S]));
+        tc_commit(smem_addr(&v_empty[s]));
       };
       for (int j = 0; j < 2 && j < ntiles; ++j) issue_qk(j);
       for (int j = 0; j < ntiles && ok; ++j) {
@@ -370,7 +423,7 @@ __global__ void __launch_bounds__(kThreads)
         if (!ok) break;
         tc_fence_after();
         issue_pv(j);
-        if (j + 2 < ntiles) issue_qk(j + 2);
+        if (ok && j + 2 < ntiles) issue_qk(j + 2);
       }
       if (!ok) {
         // every MMA issued so far has finished before tensor memory is freed
@@ -383,7 +436,6 @@ __global__ void __launch_bounds__(kThreads)
   } else {
     const int tok = threadIdx.x;  // token of the tile; head dimension of O
     const uint32_t trow = tmem + ((uint32_t)(32 * warp) << 16);
-    const uint32_t toff = ((uint32_t)(tok >> 4) << 4);
     float qsc[HG], m[HG], l[HG], alpha[HG], acc[L::kBoxes][HG];
 #pragma unroll
     for (int h = 0; h < HG; ++h) {
@@ -425,7 +477,7 @@ __global__ void __launch_bounds__(kThreads)
         tmem_wait_ld();
 #pragma unroll
         for (int h = 0; h < HG; ++h)
-          acc[b][h] = fmaf(acc[b][h], alpha[h], fmaf(fmaf(o[2 * HG + h], 0.0625f, o[HG + h]), 0.0625f, o[h]));
+          acc[b][h] = fmaf(acc[b][h], alpha[h], join_terms<kT, HG>(o, h));
       }
     };
     for (int j = 0; j < ntiles; ++j) {
@@ -434,8 +486,8 @@ __global__ void __launch_bounds__(kThreads)
       float ks_nxt, vs_nxt;
       scales_of(id_nxt, ks_nxt, vs_nxt);
       const bool vzero = vs == 0.f;
-      const float lv = vzero ? 0.f : log2f(vs);
-      const float vinv = vzero ? 1.f : 1.f / vs;
+      const float lv = vzero ? 0.f : __log2f(vs);
+      const float vinv = vzero ? 1.f : __fdividef(1.f, vs);
 
       ok = mbar_wait_bounded(smem_addr(&s_full[j & 1]), (uint32_t)(j >> 1) & 1u, a.wait_limit_ns);
       if (!__all_sync(0xffffffffu, ok)) {
@@ -450,7 +502,7 @@ __global__ void __launch_bounds__(kThreads)
       float* tops = smax + (j & 1) * 4 * L::kMaxHeads;
 #pragma unroll
       for (int h = 0; h < HG; ++h) {
-        const float s = fmaf(fmaf(x[2 * HG + h], 0.0625f, x[HG + h]), 0.0625f, x[h]);
+        const float s = join_terms<kT, HG>(x, h);
         x[h] = valid ? fmaf(s, qsc[h] * ks, lv) : -INFINITY;
         const float w = warp_max(x[h]);
         if (lane == 0) tops[warp * L::kMaxHeads + h] = w;
@@ -462,7 +514,6 @@ __global__ void __launch_bounds__(kThreads)
         ok = false;
         break;
       }
-      uint8_t* pb = smem + L::kPOff + (j & 1) * L::kQBox + (tok & 15);
       float alpha_new[HG];
 #pragma unroll
       for (int h = 0; h < HG; ++h) {
@@ -475,23 +526,38 @@ __global__ void __launch_bounds__(kThreads)
         x[h] = ex2_approx(x[h] - mu);
         l[h] = fmaf(l[h], alpha_new[h], x[h] * vinv);
       }
+      // P's bytes: column t HG + h is term t of head h
+      uint16_t pairs[N / 2];
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) pairs[i] = 0;
+      const float ps = vzero ? 0.f : kPScale;
 #pragma unroll
       for (int h = 0; h < HG; h += 2) {
-        uint16_t t[3];
-        const float ps = vzero ? 0.f : kPScale;
-        three_terms(x[h] * ps, h + 1 < HG ? x[h + 1 < HG ? h + 1 : h] * ps : 0.f, t);
+        uint16_t t[kT];
+        split_terms<kT>(__floats2half2_rn(x[h] * ps, h + 1 < HG ? x[h + 1 < HG ? h + 1 : h] * ps : 0.f), t);
 #pragma unroll
-        for (int k = 0; k < 3; ++k) {
-          const int n = k * HG + h;
-          pb[n * 128 + (toff ^ ((n & 7) << 4))] = (uint8_t)t[k];
-          if (h + 1 < HG) pb[(n + 1) * 128 + (toff ^ (((n + 1) & 7) << 4))] = (uint8_t)(t[k] >> 8);
+        for (int k = 0; k < kT; ++k) {
+          const int c = k * HG + h;
+          if (HG % 2 == 0)
+            pairs[c / 2] = t[k];
+          else  // one head: terms in neighbouring columns
+            pairs[c / 2] |= (uint16_t)((t[k] & 0xffu) << (8 * (c & 1)));
         }
+      }
+      uint4* pb = reinterpret_cast<uint4*>(smem + L::kPOff + (j & 1) * L::kPBytes) + tok;
+#pragma unroll
+      for (int c = 0; c < N / 16; ++c) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          w[i] = (uint32_t)pairs[c * 8 + 2 * i] | ((uint32_t)pairs[c * 8 + 2 * i + 1] << 16);
+        pb[c * kTile] = make_uint4(w[0], w[1], w[2], w[3]);
       }
       if (!valid) {
         // A V row that no token of the row owns (past the context, or a
         // rejected block's) may hold any bytes, and 0 * NaN is not 0.
-        mbar_wait_bounded(smem_addr(&full[j % S]), (uint32_t)(j / S) & 1u, a.wait_limit_ns);
-        uint8_t* v = smem + (j % S) * L::kStage + L::kHalf + tok * 128;
+        mbar_wait_bounded(smem_addr(&v_full[j % S]), (uint32_t)(j / S) & 1u, a.wait_limit_ns);
+        uint8_t* v = smem + L::kVOff + (j % S) * L::kHalf + tok * 128;
 #pragma unroll
         for (int b = 0; b < L::kBoxes; ++b)
 #pragma unroll
@@ -594,7 +660,7 @@ cf_status ensure_smem() {
   static std::once_flag flags[64];
   static cudaError_t errs[64];
   auto kern = block_attention_kernel<T, D, HG>;
-  constexpr int bytes = Layout<D, HG>::kAlloc;
+  constexpr int bytes = Layout<T, D, HG>::kAlloc;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_status(e);
@@ -618,7 +684,7 @@ cf_status launch_heads(Args a, const cf_paged_attention_params& p, cudaStream_t 
   cf_status st = ensure_smem<T, D, HG>();
   if (st != CF_OK) return st;
   const dim3 grid((unsigned)a.num_parts, (unsigned)(p.num_kv_heads * a.head_chunks), (unsigned)p.num_seqs);
-  block_attention_kernel<T, D, HG><<<grid, kThreads, Layout<D, HG>::kAlloc, stream>>>(a, mk, mv);
+  block_attention_kernel<T, D, HG><<<grid, kThreads, Layout<T, D, HG>::kAlloc, stream>>>(a, mk, mv);
   return check_launch();
 }
 
