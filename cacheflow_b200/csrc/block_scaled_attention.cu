@@ -26,6 +26,9 @@ namespace {
 constexpr int kBlk = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 
+// One launch's work is the tiles (128 tokens) of every (row, KV head [, head
+// chunk]) item, rows outermost, laid end to end; CTA c of G takes the tiles
+// [c W / G, (c + 1) W / G) of their W, whatever items they belong to.
 struct Args {
   const void* q;
   const float* ks;
@@ -33,19 +36,25 @@ struct Args {
   void* out;
   const int32_t* tables;
   const int32_t* lens;
-  float* part_max;  // [S, H, P] log2 units; null when unsplit
+  // Results of items that several CTAs share: CTA c's first piece in slot 2c,
+  // an item begun but not finished in 2c + 1.  Null: no item is shared, CTA c
+  // takes the items that begin in its tiles.
+  int4* meta;        // [G]: row, KV head and chunk, last CTA of the item begun (row -1: none)
+  float* part_max;   // [2 G, HG] log2 units
   float* part_sum;
-  float* part_out;  // [S, H, P, D]
+  float* part_out;   // [2 G, HG, D]
   float scale_log2;
-  int32_t num_heads, num_kv_heads, group;
+  int32_t num_seqs, num_heads, num_kv_heads, group;
   int32_t max_blocks;
-  int32_t head_chunks;  // CTAs per KV head
-  int32_t part_tokens;  // a multiple of 128
-  int32_t num_parts;
+  int32_t head_chunks;  // items per (row, KV head)
   int64_t num_blocks;
-  uint64_t wait_limit_ns;      // of every pipeline wait
-  int32_t unarm_first_stage;   // test hook (cf_testing_set_pipeline_faults)
+  uint64_t wait_limit_ns;     // of every pipeline wait
+  int32_t unarm_first_stage;  // test hook (cf_testing_set_pipeline_faults)
 };
+
+constexpr int kTile = 128;                 // tokens of a tile
+constexpr int kTileBlocks = kTile / kBlk;  // 8
+constexpr int kBox = kTile * 128;          // 128 rows x 128 bytes
 
 __device__ __forceinline__ int context_of(const Args& a, int seq, bool report) {
   const int ctx = a.lens[seq];
@@ -57,9 +66,32 @@ __device__ __forceinline__ int context_of(const Args& a, int seq, bool report) {
   return ctx;
 }
 
+// A CTA's way through its tiles, one segment (a run of tiles of one item) at
+// a time.  Every role walks its own copy.
+struct Cursor {
+  int seq, item;  // row; KV head * chunks + chunk
+  int ctx, tiles; // of the row
+  int tile;       // first tile of the segment
+  int64_t left;   // tiles of the CTA from here on
+  __device__ __forceinline__ int count() const { return (int)(left < tiles - tile ? left : (int64_t)(tiles - tile)); }
+  __device__ __forceinline__ bool done() const { return left <= 0; }
+  __device__ __forceinline__ void next(const Args& a) {
+    left -= count();
+    tile = 0;
+    if (left <= 0) return;
+    if (++item == a.num_kv_heads * a.head_chunks) {
+      item = 0;
+      do {
+        ++seq;
+        ctx = context_of(a, seq, false);
+      } while (ctx == 0);  // left > 0: a row with tiles follows
+      tiles = (ctx + kTile - 1) / kTile;
+    }
+  }
+};
+
 // ---------------------------------------------------------------------------
-// The streaming kernel: one CTA per (partition, KV head [x head chunk], row),
-// tiles of 128 tokens (8 blocks) of one KV head.
+// The streaming kernel, 1 to 3 CTAs per SM for the whole launch.
 //
 // Both products run on the stored bytes, tcgen05 kind::f8f6f4 with f32
 // accumulation in tensor memory, the tokens or head dimensions as the 128
@@ -67,27 +99,28 @@ __device__ __forceinline__ int context_of(const Args& a, int seq, bool report) {
 //   S[128 tokens x N] = K . Q^T      A = K tile (K-major), B = Q
 //   O[128 dims   x N] = V^T . P^T    A = V tile (MN-major), B = P
 // so no cached byte passes through a register.  Q and P, which e4m3 alone
-// would round to 4 bits, are three e4m3 terms each, in three of the N columns
-// per head: x = t1 + t2 / 16 + t3 / 256, every term the rounding of 16 times
-// what the ones before it leave (13 significant bits; bf16 queries are
-// exact).  Q is brought under 448 by a power of two for each head, P lies in
-// [0, 256].  The block scales join outside: ks on a token's logit, vs in its
-// weight's exponent.
+// would round to 4 bits, are two or three e4m3 terms each, in as many of the
+// N columns per head: x = t1 + t2 / 16 + t3 / 256, every term the rounding of
+// 16 times what the ones before it leave.  Q is brought under 448 by a power
+// of two for each head, P lies in [0, 256].  The block scales join outside:
+// ks on a token's logit, vs in its weight's exponent.
 //
-// Roles: warp 4 issues the TMA copies (2 KB boxes of 16 tokens x 128 bytes,
-// 128-byte swizzle) into a ring of stages, one thread of warp 5 the MMAs, and
-// warps 0-3 do the softmax: thread t has token t of each tile, reads its N
+// Roles: warps 4 and 5 issue the TMA copies of K and of V (2 KB boxes of 16
+// tokens x 128 bytes, 128-byte swizzle) into rings of stages, warp 7 stages
+// the Q terms of the next segment, one thread of warp 6 issues the MMAs, and
+// warps 0-3 do the softmax: thread t has token t of each tile, reads its
 // logit terms from tensor memory, and writes its P bytes; as the owner of
 // head dimension t it reads the tile's O from tensor memory and adds it to
-// f32 registers, rescaled there when the maximum moved.  S, P and O are
-// double-buffered: the MMAs of a tile run under the softmax of the next.
+// f32 registers, rescaled there when the maximum moved.  The copies run on
+// across segments, QK runs two tiles ahead of PV (S is double-buffered), and
+// a tile's PV runs under the next tile's logits, whose warps add its O while
+// they wait for each other's maxima.
 // ---------------------------------------------------------------------------
-constexpr int kTile = 128;                 // tokens of a tile
-constexpr int kTileBlocks = kTile / kBlk;  // 8
-constexpr int kBox = kTile * 128;          // 128 rows x 128 bytes
-constexpr int kThreads = 192;
-constexpr int kProducerWarp = 4;
-constexpr int kMmaWarp = 5;
+constexpr int kThreads = 256;  // two warpgroups: softmax, and the rest
+constexpr int kKWarp = 4;
+constexpr int kVWarp = 5;
+constexpr int kMmaWarp = 6;
+constexpr int kQWarp = 7;
 constexpr float kPScale = 256.f;
 
 // e4m3 terms of a query element and of a weight: two hold a bf16's 8
@@ -102,29 +135,40 @@ struct Layout {
   static constexpr int kHalf = kBoxes * kBox;         // a tile's K or V
   // K and V have rings of their own: a K stage is free once its QK is done,
   // a V stage an exchange of maxima and a PV later.
-  static constexpr bool kThree = D == 128 && kN == 16;  // three CTAs per SM
-  static constexpr int kStages = kThree ? 2 : 3;
+  static constexpr int kMinCtas = D == 128 ? (HG <= 8 ? 3 : 2) : 1;  // per SM
+  static constexpr int kStages = kMinCtas == 3 ? 2 : 3;
+  // Registers of a softmax thread, and of the others, where the launch's even
+  // share (80 at three CTAs per SM, 128 at two) is too few: what one
+  // warpgroup gives up is at least what the other takes.
+  static constexpr bool kSplitRegs = D == 128 && HG >= 8;
+  static constexpr int kLaunchRegs = kMinCtas == 3 ? 80 : 128;
+  static constexpr int kSoftmaxRegs = kMinCtas == 3 ? 112 : 200;
+  static constexpr int kOtherRegs = kMinCtas == 3 ? 48 : 56;
+  static_assert(kSoftmaxRegs + kOtherRegs <= 2 * kLaunchRegs, "more registers than the block has");
   static constexpr int kVOff = kStages * kHalf;
   static constexpr int kQOff = 2 * kStages * kHalf;   // Q: kBoxes x [kN rows x 128 B]
   static constexpr int kQBox = kN * 128;
-  static constexpr int kPOff = kQOff + kBoxes * kQBox;  // P: 2 x [kN/16 planes x 128 tokens x 16 B]
-  static constexpr int kPBytes = kN * 128;
-  static constexpr int kBarOff = kPOff + 2 * kPBytes;
-  // full, empty of K and of V; s_full, p_full, o_full, top by tile parity; fin
-  static constexpr int kNumBars = 4 * kStages + 4 * 2 + 1;
-  static constexpr int kMaxOff = kBarOff + (kNumBars * 8 + 15) / 16 * 16;  // [2][4][HG] f32
+  static constexpr int kPOff = kQOff + kBoxes * kQBox;  // P: kN/16 planes x 128 tokens x 16 B
+  static constexpr int kBarOff = kPOff + kN * 128;
+  // full, empty of K and of V; s_full and top by tile parity; p_full, o_full,
+  // q_full, q_empty, sums, fin
+  static constexpr int kNumBars = 4 * kStages + 2 * 2 + 6;
+  static constexpr int kScaleOff = kBarOff + (kNumBars * 8 + 15) / 16 * 16;  // [stages][ks 8, vs 8] f32
+  static constexpr int kMaskOff = kScaleOff + kStages * 2 * kTileBlocks * 4;  // [stages] int
+  static constexpr int kMaxOff = kMaskOff + 16;                               // [2][4][HG] f32
   static constexpr int kMaxHeads = (HG + 3) / 4 * 4;
   static constexpr int kSumOff = kMaxOff + 2 * 4 * kMaxHeads * 4;          // [4][HG] f32
   static constexpr int kQsOff = kSumOff + 4 * kMaxHeads * 4;               // [HG] f32
-  static constexpr int kOkOff = kQsOff + kMaxHeads * 4;                     // [4] int
-  static constexpr int kTmemOff = kOkOff + 16;
+  static constexpr int kStartOff = kQsOff + kMaxHeads * 4;                  // Cursor
+  static constexpr int kScanOff = kStartOff + 32;                           // [8 warps + 1] int64
+  static constexpr int kTmemOff = kScanOff + 80;
   static constexpr int kBytes = kTmemOff + 16;
   static constexpr int kAlloc = kBytes + 1024;
-  static constexpr int kMinCtas = kThree ? 3 : (D == 128 ? 2 : 1);
   static constexpr int kOCol = 2 * kN;                 // O after the two S buffers
-  static constexpr int kCols = 2 * kN + 2 * kBoxes * kN;
+  static constexpr int kCols = 2 * kN + kBoxes * kN;
   static constexpr uint32_t kTmemCols = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
-  static_assert(kAlloc <= 227 * 1024, "shared memory of one CTA");
+  static_assert(kStages <= 4, "mask words");
+  static_assert(kMinCtas * (kAlloc + 1024) <= 228 * 1024 && kMinCtas * kTmemCols <= 512, "CTAs per SM");
 };
 
 // Instruction descriptor of kind::f8f6f4: f32 accumulation, A and B e4m3,
@@ -158,6 +202,27 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
       : "r"(taddr));
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// mbar_wait_bounded with the barrier unit asked to hold the thread for up to
+// 2 us per try: warps that wait for another role leave the issue slots to it.
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
+  const uint32_t b = smem_addr(bar);
+  uint64_t t0 = 0;
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(b), "r"(parity), "r"(2000u)
+        : "memory");
+    if (ok) return true;
+    const uint64_t t = global_timer_ns();
+    if (t0 == 0) t0 = t;
+    if (t - t0 > limit_ns) return false;
+  }
 }
 
 // Max over the warp; a NaN takes no part.
@@ -195,28 +260,84 @@ __device__ __forceinline__ float join_terms(const float* v, int h) {
   return r;
 }
 
+// The CTA's first tile and how many it has, found by all threads: prefix sums
+// of the rows' tiles, then the thread whose rows hold the tile walks them.
+template <typename L>
+__device__ __forceinline__ Cursor find_start(const Args& a, uint8_t* smem) {
+  Cursor* start = reinterpret_cast<Cursor*>(smem + L::kStartOff);
+  int64_t* scan = reinterpret_cast<int64_t*>(smem + L::kScanOff);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t items = (int64_t)a.num_kv_heads * a.head_chunks;
+  const int per = (a.num_seqs + kThreads - 1) / kThreads;
+  const int s0 = min(a.num_seqs, (int)threadIdx.x * per), s1 = min(a.num_seqs, s0 + per);
+  int64_t sum = 0;
+  for (int s = s0; s < s1; ++s) sum += (context_of(a, s, blockIdx.x == 0) + kTile - 1) / kTile;
+  int64_t incl = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) scan[warp] = incl;
+  if (threadIdx.x == 0) *start = Cursor{0, 0, 0, 0, 0, 0};
+  __syncthreads();
+  int64_t before = incl - sum, total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += scan[w];
+    total += scan[w];
+  }
+  // no more CTAs than tiles take part, so each of them has at least one
+  const int64_t W = total * items, G = W < gridDim.x ? (W > 0 ? W : 1) : gridDim.x;
+  const int64_t b0 = blockIdx.x < G ? W * blockIdx.x / G : W, b1 = blockIdx.x < G ? W * (blockIdx.x + 1) / G : W;
+  const bool whole = a.meta == nullptr;  // items are not shared: both ends move on to where one begins
+  __syncthreads();  // the scan words have been read: they become the two ends
+  if (threadIdx.x == 0) {
+    scan[0] = b0;
+    scan[1] = b1;
+    scan[2] = W;
+    scan[3] = G;
+  }
+  __syncthreads();
+  // tile b lies in the row with items * before <= b < items * (before + its tiles)
+  for (int e = 0; e < (whole ? 2 : 1); ++e) {
+    const int64_t b = e == 0 ? b0 : b1;
+    if (b < items * before || b >= items * (before + sum)) continue;
+    int64_t at = before;
+    for (int s = s0; s < s1; ++s) {
+      const int ctx = context_of(a, s, false);
+      const int n = (ctx + kTile - 1) / kTile;
+      if (b < items * (at + n)) {
+        const int64_t off = b - items * at;
+        const int64_t up = whole ? (n - off % n) % n : 0;
+        if (e == 0) *start = Cursor{s, (int)((off + up) / n), ctx, n, (int)((off + up) % n), 0};
+        scan[e] = b + up;
+        break;
+      }
+      at += n;
+    }
+  }
+  __syncthreads();
+  Cursor c = *start;
+  c.left = scan[1] - scan[0];
+  if (c.left > 0 && c.item == items) {  // moved on past the row's last item
+    c.item = 0;
+    do {
+      ++c.seq;
+      c.ctx = context_of(a, c.seq, false);
+    } while (c.ctx == 0);
+    c.tiles = (c.ctx + kTile - 1) / kTile;
+  }
+  return c;
+}
+
 template <typename T, int D, int HG>
 __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
     block_attention_kernel(const Args a, const __grid_constant__ CUtensorMap tmk,
                            const __grid_constant__ CUtensorMap tmv) {
   using L = Layout<T, D, HG>;
   constexpr int N = L::kN, S = L::kStages, kT = kTerms<T>;
-  const int part = blockIdx.x, seq = blockIdx.z;
-  const int kvh = blockIdx.y / a.head_chunks, chunk = blockIdx.y - kvh * a.head_chunks;
-  const int head0 = kvh * a.group + chunk * HG;
-  const int nheads = min(HG, a.group - chunk * HG);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int ctx = context_of(a, seq, threadIdx.x == 0 && part == 0 && blockIdx.y == 0);
-  const int nparts = ctx == 0 ? 1 : (ctx + a.part_tokens - 1) / a.part_tokens;
-  if (part >= nparts) return;
-  if (part == 0 && nparts > (int)gridDim.x && threadIdx.x == 0 && blockIdx.y == 0)
-    block_attn_error(CF_DEVERR_CONTEXT_LEN);  // context_lens exceeds max_context_len
-  const bool single = nparts == 1;
-  const int t0 = part * a.part_tokens;
-  const int ntok = min(a.part_tokens, ctx - t0);  // of this partition; 0 for an empty row
-  const int ntiles = (ntok + kTile - 1) / kTile;
-  const int nblk = (ntok + kBlk - 1) / kBlk;
-  const int32_t* table = a.tables + (size_t)seq * a.max_blocks + t0 / kBlk;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -225,170 +346,226 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
   uint64_t* k_empty = bars + S;
   uint64_t* v_full = bars + 2 * S;
   uint64_t* v_empty = bars + 3 * S;
-  uint64_t* s_full = bars + 4 * S;  // [2], by tile parity, as the ones below
-  uint64_t* p_full = s_full + 2;
-  uint64_t* o_full = p_full + 2;
-  uint64_t* top = o_full + 2;
-  uint64_t* fin = top + 2;
+  uint64_t* s_full = bars + 4 * S;  // [2], by tile parity, as top
+  uint64_t* top = s_full + 2;
+  uint64_t* p_full = top + 2;
+  uint64_t* o_full = p_full + 1;
+  uint64_t* q_full = o_full + 1;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* sums = q_empty + 1;
+  uint64_t* fin = sums + 1;
+  float* scales = reinterpret_cast<float*>(smem + L::kScaleOff);
+  int* masks = reinterpret_cast<int*>(smem + L::kMaskOff);
   float* smax = reinterpret_cast<float*>(smem + L::kMaxOff);
   float* ssum = reinterpret_cast<float*>(smem + L::kSumOff);
   float* sqs = reinterpret_cast<float*>(smem + L::kQsOff);
-  int* sok = reinterpret_cast<int*>(smem + L::kOkOff);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kTmemOff);
 
-  int ids = 0, ids_next = 0;  // producer: block ids of this and the next 32 blocks
-  auto load_ids = [&](int b) { return b + lane < nblk ? table[b + lane] : 0; };
-  int id = 0;
-  bool valid_id = false;
-  auto produce_k = [&](int j) {  // takes the tile's ids, then copies K
-    const int b0 = j * kTileBlocks;
-    if ((b0 & 31) == 0) {
-      ids = b0 == 0 ? load_ids(0) : ids_next;
-      ids_next = load_ids(b0 + 32);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(smem_addr(&k_full[s]), 1);
+      mbar_init(smem_addr(&k_empty[s]), 1);
+      mbar_init(smem_addr(&v_full[s]), 1 + 2 * kTileBlocks);  // V's bytes, and 16 lanes' scales
+      mbar_init(smem_addr(&v_empty[s]), 1);
     }
-    id = __shfl_sync(0xffffffffu, ids, (b0 & 31) + (lane & 7));
-    const bool want = lane < kTileBlocks && b0 + lane < nblk;
-    valid_id = want && id >= 0 && (int64_t)id < a.num_blocks;
-    if (want && !valid_id) block_attn_error(CF_DEVERR_BLOCK_ID);
-  };
-  // Copies the tile's K or V: lane k block k, onto the stage's barrier.
-  auto copy = [&](int j, const CUtensorMap* map, uint64_t* full, uint8_t* ring) {
-    if (a.unarm_first_stage && j == 0) return;  // test hook: the stage never completes
-    const uint32_t bar = smem_addr(&full[j % S]);
-    const uint32_t mask = __ballot_sync(0xffffffffu, valid_id);
-    if (lane == 0) {
-      fence_proxy_async_smem();
-      if (mask == 0)
-        mbar_arrive(bar);
-      else
-        mbar_arrive_expect_tx(bar, (uint32_t)__popc(mask) * kBlk * D);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_addr(&s_full[i]), 1);
+      mbar_init(smem_addr(&top[i]), 4);
     }
-    __syncwarp();
-    if (valid_id) {
-      const int32_t row = (int32_t)(((int64_t)id * a.num_kv_heads + kvh) * kBlk);
-      uint8_t* dst = ring + (j % S) * L::kHalf + lane * (kBlk * 128);
-#pragma unroll
-      for (int b = 0; b < L::kBoxes; ++b) tma_load_2d(smem_addr(dst + b * kBox), map, b * 128, row, bar);
-    }
-    __syncwarp();
-  };
-  auto produce = [&](int j) {
-    produce_k(j);
-    copy(j, &tmk, k_full, smem);
-    copy(j, &tmv, v_full, smem + L::kVOff);
-  };
-
-  // Set-up: the producer starts copying as soon as the barriers are there;
-  // Q's terms and the tensor memory follow beside it.
-  int produced = 0;
-  if (warp == kProducerWarp) {
-    if (lane == 0) {
-      for (int s = 0; s < S; ++s) {
-        mbar_init(smem_addr(&k_full[s]), 1);
-        mbar_init(smem_addr(&k_empty[s]), 1);
-        mbar_init(smem_addr(&v_full[s]), 1);
-        mbar_init(smem_addr(&v_empty[s]), 1);
-      }
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(smem_addr(&s_full[i]), 1);
-        mbar_init(smem_addr(&p_full[i]), kTile);
-        mbar_init(smem_addr(&o_full[i]), 1);
-        mbar_init(smem_addr(&top[i]), 4);
-      }
-      mbar_init(smem_addr(fin), 1);
-      fence_mbar_init();
-    }
-    __syncwarp();
-    for (; produced < ntiles && produced < S; ++produced) produce(produced);
-  } else if (warp == kMmaWarp) {
+    mbar_init(smem_addr(p_full), kTile);
+    mbar_init(smem_addr(o_full), 1);
+    mbar_init(smem_addr(q_full), 32);
+    mbar_init(smem_addr(q_empty), 1 + 4);  // its last QK, and the softmax warps' reads of the scales
+    mbar_init(smem_addr(sums), 4);
+    mbar_init(smem_addr(fin), 1);
+    fence_mbar_init();
+  }
+  if (warp == kMmaWarp) {
     tmem_alloc(smem_addr(tmem_slot), L::kTmemCols);
     tmem_relinquish();
-  } else {
-    constexpr int E = D / 32;
-    for (int n = warp; n < N; n += 4) {  // rows past the terms
-      if (n >= kT * HG)
-        for (int b = 0; b < L::kBoxes; ++b)
-          reinterpret_cast<uint32_t*>(smem + L::kQOff + b * L::kQBox + n * 128)[lane] = 0u;
-    }
-    for (int h = warp; h < HG; h += 4) {
-      float q[E];
-#pragma unroll
-      for (int e = 0; e < E; ++e) q[e] = 0.f;
-      if (h < nheads)
-        load_widen<T, E>(static_cast<const T*>(a.q) + ((size_t)seq * a.num_heads + head0 + h) * D + lane * E, q);
-      float mx = 0.f;
-      bool bad = false;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const bool fin = fabsf(q[e]) <= 3.402823466e38f;
-        bad = bad || !fin;
-        mx = fmaxf(mx, fin ? fabsf(q[e]) : 0.f);
-      }
-      mx = warp_max(mx);
-      bad = __any_sync(0xffffffffu, bad);
-      // the smallest power of two s with mx <= 448 s (448 = 1.75 * 2^8)
-      const uint32_t bits = __float_as_uint(mx);
-      int ex = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-      ex = mx == 0.f ? 127 : (ex < 1 ? 1 : ex);
-      const float inv = __uint_as_float((uint32_t)(254 - ex) << 23);
-#pragma unroll
-      for (int e = 0; e < E; e += 4) {
-        uint16_t lo[kT], hi[kT];
-        split_terms<kT>(__floats2half2_rn(q[e] * inv, q[e + 1] * inv), lo);
-        split_terms<kT>(__floats2half2_rn(q[e + 2] * inv, q[e + 3] * inv), hi);
-        const int col = lane * E + e;  // byte of the row
-#pragma unroll
-        for (int t = 0; t < kT; ++t) {
-          const int n = t * HG + h;
-          uint32_t w = (uint32_t)lo[t] | ((uint32_t)hi[t] << 16);
-          if (bad) w = 0x7f7f7f7fu;  // a query that is not finite has no softmax: NaN
-          *reinterpret_cast<uint32_t*>(smem + L::kQOff + (col >> 7) * L::kQBox + n * 128 +
-                                       ((((col >> 4) & 7) ^ (n & 7)) << 4) + (col & 15)) = w;
-        }
-      }
-      if (lane == 0) sqs[h] = __uint_as_float((uint32_t)ex << 23);
-    }
-    fence_proxy_async_smem();
   }
   tc_fence_before();
-  __syncthreads();
+  Cursor cur = find_start<L>(a, smem);  // synchronises the block
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  const int64_t ntiles = cur.left;  // of this CTA
 
-  if (warp == kProducerWarp) {
-    bool ok = true;
-    for (; produced < ntiles; ++produced) {
-      const int s = produced % S;
-      const uint32_t parity = (uint32_t)(produced / S - 1) & 1u;
-      produce_k(produced);
-      ok = mbar_wait_bounded(smem_addr(&k_empty[s]), parity, a.wait_limit_ns);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      copy(produced, &tmk, k_full, smem);
-      ok = mbar_wait_bounded(smem_addr(&v_empty[s]), parity, a.wait_limit_ns);
-      if (!__all_sync(0xffffffffu, ok)) {
-        if (lane == 0) mbar_wait_bounded(smem_addr(&k_full[s]), (uint32_t)(produced / S) & 1u, a.wait_limit_ns);
-        break;
-      }
-      copy(produced, &tmv, v_full, smem + L::kVOff);
+  // Rows without a context: zeros, dealt to the CTAs in turn.
+  for (int s = blockIdx.x; s < a.num_seqs; s += gridDim.x)
+    if (context_of(a, s, false) == 0) {
+      T* o = static_cast<T*>(a.out) + (size_t)s * a.num_heads * D;
+      for (int i = threadIdx.x; i < a.num_heads * D; i += kThreads) o[i] = from_float<T>(0.f);
     }
-    if (!ok) block_attn_error(CF_DEVERR_TIMEOUT);
-    // no copy may land after the CTA has left
-    if (lane == 0)
-      for (int j = produced > S ? produced - S : 0; j < produced; ++j) {
-        mbar_wait_bounded(smem_addr(&k_full[j % S]), (uint32_t)(j / S) & 1u, a.wait_limit_ns);
-        mbar_wait_bounded(smem_addr(&v_full[j % S]), (uint32_t)(j / S) & 1u, a.wait_limit_ns);
+
+  if (warp >= 4) {
+    if constexpr (L::kSplitRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kOtherRegs));
+    if (warp == kKWarp || warp == kVWarp) {
+      // ---------------- copies of K, or of V with the scales ----------------
+      const bool is_k = warp == kKWarp;
+      uint64_t* fulls = is_k ? k_full : v_full;
+      uint64_t* empties = is_k ? k_empty : v_empty;
+      uint8_t* ring = smem + (is_k ? 0 : L::kVOff);
+      const CUtensorMap* map = is_k ? &tmk : &tmv;
+      bool ok = true;
+      int64_t j = 0;  // tiles begun
+      // Block ids come 32 (four tiles) at a time, a group ahead of their use:
+      // `ahead` stands at the group whose ids are in `ids_next`.
+      Cursor ahead = cur;
+      int at = 0;  // tile of `ahead`'s segment
+      auto fetch = [&]() {
+        if (ahead.done()) return 0;
+        const int b = (ahead.tile + at) * kTileBlocks + lane;
+        const int last = min((ahead.ctx + kBlk - 1) / kBlk, (ahead.tile + ahead.count()) * kTileBlocks);
+        return b < last ? a.tables[(size_t)ahead.seq * a.max_blocks + b] : 0;
+      };
+      auto step = [&]() {
+        at += 4;
+        if (at >= ahead.count()) {
+          at = 0;
+          ahead.next(a);
+        }
+      };
+      int ids_next = fetch();
+      for (; !cur.done() && ok; cur.next(a)) {
+        const int cnt = cur.count(), nblk = (cur.ctx + kBlk - 1) / kBlk;
+        const int kvh = cur.item / a.head_chunks;
+        int ids = 0;
+        for (int i = 0; i < cnt; ++i, ++j) {
+          if ((i & 3) == 0) {
+            ids = ids_next;
+            step();
+            ids_next = fetch();
+          }
+          const int s = (int)(j % S);
+          const int k = lane & 7;
+          const int id = __shfl_sync(0xffffffffu, ids, (i & 3) * kTileBlocks + k);
+          const bool want = (cur.tile + i) * kTileBlocks + k < nblk;
+          const bool valid = want && id >= 0 && (int64_t)id < a.num_blocks;
+          if (want && !valid && lane < kTileBlocks) block_attn_error(CF_DEVERR_BLOCK_ID);
+          const uint32_t mask = __ballot_sync(0xffffffffu, valid) & 0xffu;
+          if (j >= S) {
+            ok = wait_bar(&empties[s], (uint32_t)(j / S - 1) & 1u, a.wait_limit_ns);
+            if (!__all_sync(0xffffffffu, ok)) {
+              ok = false;
+              break;
+            }
+          }
+          if (a.unarm_first_stage && j == 0) continue;  // test hook: the stage never completes
+          const uint32_t bar = smem_addr(&fulls[s]);
+          if (lane == 0) {
+            if (!is_k) masks[s] = (int)mask;
+            fence_proxy_async_smem();
+            if (mask == 0)
+              mbar_arrive(bar);
+            else
+              mbar_arrive_expect_tx(bar, (uint32_t)__popc(mask) * kBlk * D);
+          }
+          __syncwarp();
+          if (valid && lane < kTileBlocks) {  // lane k copies block k
+            const int32_t row = (int32_t)(((int64_t)id * a.num_kv_heads + kvh) * kBlk);
+            uint8_t* dst = ring + s * L::kHalf + lane * (kBlk * 128);
+#pragma unroll
+            for (int b = 0; b < L::kBoxes; ++b) tma_load_2d(smem_addr(dst + b * kBox), map, b * 128, row, bar);
+          }
+          if (!is_k && lane < 2 * kTileBlocks) {  // lanes 0-7 a block's ks, 8-15 its vs
+            if (valid)
+              cp_async4(smem_addr(&scales[s * 2 * kTileBlocks + lane]),
+                        (lane < kTileBlocks ? a.ks : a.vs) + (int64_t)id * a.num_kv_heads + kvh);
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+          }
+          __syncwarp();
+        }
       }
-  } else if (warp == kMmaWarp) {
-    if (lane == 0) {
+      if (!ok) block_attn_error(CF_DEVERR_TIMEOUT);
+      // no copy may land after the CTA has left
+      cp_async_wait_all();
+      if (lane == 0)
+        for (int64_t i = j > S ? j - S : 0; i < j; ++i)
+          wait_bar(&fulls[i % S], (uint32_t)(i / S) & 1u, a.wait_limit_ns);
+    } else if (warp == kQWarp) {
+      // ---------------- Q's terms, a segment at a time ----------------
+      constexpr int E = D / 32;
+      constexpr int kBatch = HG < 8 ? HG : 8;  // heads whose loads run before the wait
+      for (int n = kT * HG; n < N; ++n)  // rows past the terms
+        for (int b = 0; b < L::kBoxes; ++b)
+          reinterpret_cast<uint32_t*>(smem + L::kQOff + b * L::kQBox + n * 128)[lane] = 0u;
+      bool ok = true;
+      for (int seg = 0; !cur.done() && ok; cur.next(a), ++seg) {
+        const int kvh = cur.item / a.head_chunks, chunk = cur.item - kvh * a.head_chunks;
+        const int head0 = kvh * a.group + chunk * HG, nheads = min(HG, a.group - chunk * HG);
+        const T* src = static_cast<const T*>(a.q) + ((size_t)cur.seq * a.num_heads + head0) * D + lane * E;
+#pragma unroll
+        for (int h0 = 0; h0 < HG; h0 += kBatch) {
+          uint32_t raw[kBatch][E / 2];
+#pragma unroll
+          for (int h = 0; h < kBatch; ++h)
+#pragma unroll
+            for (int e = 0; e < E / 2; ++e)
+              raw[h][e] = h0 + h < nheads ? reinterpret_cast<const uint32_t*>(src + (size_t)(h0 + h) * D)[e] : 0u;
+          if (h0 == 0 && seg > 0) {
+            ok = wait_bar(q_empty, (uint32_t)(seg - 1) & 1u, a.wait_limit_ns);
+            if (!__all_sync(0xffffffffu, ok)) {
+              ok = false;
+              break;
+            }
+          }
+#pragma unroll
+          for (int hb = 0; hb < kBatch; ++hb) {
+            const int h = h0 + hb;
+            float q[E];
+            float mx = 0.f;
+            bool bad = false;
+#pragma unroll
+            for (int e = 0; e < E / 2; ++e) unpack_word<T>(raw[hb][e], q + 2 * e);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+              const bool fin = fabsf(q[e]) <= 3.402823466e38f;
+              bad = bad || !fin;
+              mx = fmaxf(mx, fin ? fabsf(q[e]) : 0.f);
+            }
+            mx = warp_max(mx);
+            bad = __any_sync(0xffffffffu, bad);
+            // the smallest power of two s with mx <= 448 s (448 = 1.75 * 2^8)
+            const uint32_t bits = __float_as_uint(mx);
+            int ex = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+            ex = mx == 0.f ? 127 : (ex < 1 ? 1 : ex);
+            const float inv = __uint_as_float((uint32_t)(254 - ex) << 23);
+#pragma unroll
+            for (int e = 0; e < E; e += 4) {
+              uint16_t lo[kT], hi[kT];
+              split_terms<kT>(__floats2half2_rn(q[e] * inv, q[e + 1] * inv), lo);
+              split_terms<kT>(__floats2half2_rn(q[e + 2] * inv, q[e + 3] * inv), hi);
+              const int col = lane * E + e;  // byte of the row
+#pragma unroll
+              for (int t = 0; t < kT; ++t) {
+                const int n = t * HG + h;
+                uint32_t w = (uint32_t)lo[t] | ((uint32_t)hi[t] << 16);
+                if (bad) w = 0x7f7f7f7fu;  // a query that is not finite has no softmax: NaN
+                *reinterpret_cast<uint32_t*>(smem + L::kQOff + (col >> 7) * L::kQBox + n * 128 +
+                                             ((((col >> 4) & 7) ^ (n & 7)) << 4) + (col & 15)) = w;
+              }
+            }
+            if (lane == 0) sqs[h] = __uint_as_float((uint32_t)ex << 23);
+          }
+        }
+        if (!ok) break;
+        fence_proxy_async_smem();
+        mbar_arrive(smem_addr(q_full));
+      }
+      if (!ok) block_attn_error(CF_DEVERR_TIMEOUT);
+    } else if (lane == 0) {
+      // ---------------- MMA issuer ----------------
       const uint64_t k_desc = smem_desc_sw128(smem_addr(smem), 16, 1024);
       const uint64_t v_desc = smem_desc_sw128(smem_addr(smem + L::kVOff), 16, 1024);
       const uint64_t q_desc = smem_desc_sw128(smem_addr(smem + L::kQOff), 16, 1024);
       // P: 8 tokens x 16 columns per 128 bytes, tokens onward, then planes
       const uint64_t p_desc = smem_desc_plain(smem_addr(smem + L::kPOff), 128, kTile * 16);
       bool ok = true;
-      auto issue_qk = [&](int j) {
-        const int s = j % S;
-        ok = ok && mbar_wait_bounded(smem_addr(&k_full[s]), (uint32_t)(j / S) & 1u, a.wait_limit_ns);
+      int seg = 0, i = 0;  // segment and its next tile, of the next QK
+      auto issue_qk = [&](int64_t j) {
+        const int s = (int)(j % S);
+        ok = ok && (i > 0 || wait_bar(q_full, (uint32_t)seg & 1u, a.wait_limit_ns)) &&
+             wait_bar(&k_full[s], (uint32_t)(j / S) & 1u, a.wait_limit_ns);
         if (!ok) return;
         tc_fence_after();
         const uint64_t kd = k_desc + (uint64_t)((s * L::kHalf) >> 4);
@@ -396,220 +573,228 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
         for (int kk = 0; kk < D / 32; ++kk) {
           const uint64_t ad = kd + (uint64_t)(((kk >> 2) * kBox + (kk & 3) * 32) >> 4);
           const uint64_t bd = q_desc + (uint64_t)(((kk >> 2) * L::kQBox + (kk & 3) * 32) >> 4);
-          mma_f8(tmem + (j & 1) * N, ad, bd, idesc_f8(0, N), kk > 0 ? 1u : 0u);
+          mma_f8(tmem + (int)(j & 1) * N, ad, bd, idesc_f8(0, N), kk > 0 ? 1u : 0u);
         }
         tc_commit(smem_addr(&s_full[j & 1]));
         tc_commit(smem_addr(&k_empty[s]));
+        if (++i == cur.count()) {
+          tc_commit(smem_addr(q_empty));
+          i = 0;
+          ++seg;
+          cur.next(a);
+        }
       };
-      auto issue_pv = [&](int j) {
-        const int s = j % S;
-        ok = mbar_wait_bounded(smem_addr(&v_full[s]), (uint32_t)(j / S) & 1u, a.wait_limit_ns);
-        if (!ok) return;
+      for (int64_t j = 0; j < 2 && j < ntiles; ++j) issue_qk(j);
+      for (int64_t j = 0; j < ntiles && ok; ++j) {
+        const int s = (int)(j % S);
+        ok = wait_bar(p_full, (uint32_t)j & 1u, a.wait_limit_ns) &&
+             wait_bar(&v_full[s], (uint32_t)(j / S) & 1u, a.wait_limit_ns);
+        if (!ok) break;
         tc_fence_after();
         const uint64_t vd = v_desc + (uint64_t)((s * L::kHalf) >> 4);
-        const uint64_t pd = p_desc + (uint64_t)(((j & 1) * L::kPBytes) >> 4);
 #pragma unroll
         for (int b = 0; b < L::kBoxes; ++b)
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)  // 32 tokens each
-            mma_f8(tmem + L::kOCol + ((j & 1) * L::kBoxes + b) * N, vd + (uint64_t)((b * kBox + kk * 4096) >> 4),
-                   pd + (uint64_t)((kk * 512) >> 4), idesc_f8(1, N), kk > 0 ? 1u : 0u);
-        tc_commit(smem_addr(&o_full[j & 1]));
+            mma_f8(tmem + L::kOCol + b * N, vd + (uint64_t)((b * kBox + kk * 4096) >> 4),
+                   p_desc + (uint64_t)((kk * 512) >> 4), idesc_f8(1, N), kk > 0 ? 1u : 0u);
+        tc_commit(smem_addr(o_full));
         tc_commit(smem_addr(&v_empty[s]));
-      };
-      for (int j = 0; j < 2 && j < ntiles; ++j) issue_qk(j);
-      for (int j = 0; j < ntiles && ok; ++j) {
-        ok = mbar_wait_bounded(smem_addr(&p_full[j & 1]), (uint32_t)(j >> 1) & 1u, a.wait_limit_ns);
-        if (!ok) break;
-        tc_fence_after();
-        issue_pv(j);
-        if (ok && j + 2 < ntiles) issue_qk(j + 2);
+        if (j + 2 < ntiles) issue_qk(j + 2);
       }
       if (!ok) {
         // every MMA issued so far has finished before tensor memory is freed
         block_attn_error(CF_DEVERR_TIMEOUT);
         tc_commit(smem_addr(fin));
-        mbar_wait_bounded(smem_addr(fin), 0u, a.wait_limit_ns);
+        wait_bar(fin, 0u, a.wait_limit_ns);
       }
     }
     __syncwarp();
   } else {
+    // ---------------- softmax ----------------
+    if constexpr (L::kSplitRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kSoftmaxRegs));
     const int tok = threadIdx.x;  // token of the tile; head dimension of O
     const uint32_t trow = tmem + ((uint32_t)(32 * warp) << 16);
-    float qsc[HG], m[HG], l[HG], alpha[HG], acc[L::kBoxes][HG];
-#pragma unroll
-    for (int h = 0; h < HG; ++h) {
-      qsc[h] = sqs[h] * a.scale_log2;
-      m[h] = -INFINITY;
-      l[h] = 0.f;
-      alpha[h] = 0.f;
-#pragma unroll
-      for (int b = 0; b < L::kBoxes; ++b) acc[b][h] = 0.f;
-    }
-    // The scales of this thread's token, one tile ahead (the id two ahead).
-    auto id_of = [&](int j) {
-      const int b = j * kTileBlocks + (tok >> 4);
-      return b < nblk ? table[b] : -1;
-    };
-    auto scales_of = [&](int id, float& ks, float& vs) {
-      ks = vs = 0.f;
-      if (id < 0 || (int64_t)id >= a.num_blocks) return;
-      const int64_t u = (int64_t)id * a.num_kv_heads + kvh;
-      ks = a.ks[u];
-      vs = a.vs[u];
-    };
-    int id_cur = id_of(0), id_nxt = id_of(1);
-    float ks, vs;
-    scales_of(id_cur, ks, vs);
-    bool ok = true;
-    auto add_o = [&](int j) {  // the accumulator takes tile j's O
-      ok = mbar_wait_bounded(smem_addr(&o_full[j & 1]), (uint32_t)(j >> 1) & 1u, a.wait_limit_ns);
-      if (!__all_sync(0xffffffffu, ok)) {
-        ok = false;
-        return;
-      }
-      tc_fence_after();
-#pragma unroll
-      for (int b = 0; b < L::kBoxes; ++b) {
-        float o[N];
-#pragma unroll
-        for (int c = 0; c < N; c += 16) tmem_ld16(trow + L::kOCol + ((j & 1) * L::kBoxes + b) * N + c, &o[c]);
-        tmem_wait_ld();
-#pragma unroll
-        for (int h = 0; h < HG; ++h)
-          acc[b][h] = fmaf(acc[b][h], alpha[h], join_terms<kT, HG>(o, h));
-      }
-    };
-    for (int j = 0; j < ntiles; ++j) {
-      const bool valid = j * kTile + tok < ntok && id_cur >= 0 && (int64_t)id_cur < a.num_blocks;
-      const int id_nn = id_of(j + 2);
-      float ks_nxt, vs_nxt;
-      scales_of(id_nxt, ks_nxt, vs_nxt);
-      const bool vzero = vs == 0.f;
-      const float lv = vzero ? 0.f : __log2f(vs);
-      const float vinv = vzero ? 1.f : __fdividef(1.f, vs);
-
-      ok = mbar_wait_bounded(smem_addr(&s_full[j & 1]), (uint32_t)(j >> 1) & 1u, a.wait_limit_ns);
+    bool ok = true, begun = false;
+    int64_t j = 0;
+    for (int seg = 0; !cur.done(); cur.next(a), ++seg) {
+      const int cnt = cur.count();
+      const int kvh = cur.item / a.head_chunks, chunk = cur.item - kvh * a.head_chunks;
+      float qsc[HG], m[HG], l[HG], alpha[HG], acc[L::kBoxes][HG];
+      ok = wait_bar(q_full, (uint32_t)seg & 1u, a.wait_limit_ns);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
       }
-      tc_fence_after();
-      float x[N];
-#pragma unroll
-      for (int c = 0; c < N; c += 16) tmem_ld16(trow + (j & 1) * N + c, &x[c]);
-      tmem_wait_ld();
-      float* tops = smax + (j & 1) * 4 * L::kMaxHeads;
 #pragma unroll
       for (int h = 0; h < HG; ++h) {
-        const float s = join_terms<kT, HG>(x, h);
-        x[h] = valid ? fmaf(s, qsc[h] * ks, lv) : -INFINITY;
-        const float w = warp_max(x[h]);
-        if (lane == 0) tops[warp * L::kMaxHeads + h] = w;
+        qsc[h] = sqs[h] * a.scale_log2;
+        m[h] = -INFINITY;
+        l[h] = 0.f;
+        alpha[h] = 0.f;
+#pragma unroll
+        for (int b = 0; b < L::kBoxes; ++b) acc[b][h] = 0.f;
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_addr(&top[j & 1]));
-      ok = mbar_wait_bounded(smem_addr(&top[j & 1]), (uint32_t)(j >> 1) & 1u, a.wait_limit_ns);
+      if (lane == 0) mbar_arrive(smem_addr(q_empty));
+      auto add_o = [&](int64_t t) {  // the accumulator takes tile t's O
+        ok = wait_bar(o_full, (uint32_t)t & 1u, a.wait_limit_ns);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          return;
+        }
+        tc_fence_after();
+#pragma unroll
+        for (int b = 0; b < L::kBoxes; ++b) {
+          float o[N];
+#pragma unroll
+          for (int c = 0; c < N; c += 16) tmem_ld16(trow + L::kOCol + b * N + c, &o[c]);
+          tmem_wait_ld();
+#pragma unroll
+          for (int h = 0; h < HG; ++h) acc[b][h] = fmaf(acc[b][h], alpha[h], join_terms<kT, HG>(o, h));
+        }
+      };
+      for (int i = 0; i < cnt; ++i, ++j) {
+        const int par = (int)(j & 1), s = (int)(j % S);
+        ok = wait_bar(&v_full[s], (uint32_t)(j / S) & 1u, a.wait_limit_ns) &&
+             wait_bar(&s_full[par], (uint32_t)(j >> 1) & 1u, a.wait_limit_ns);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const bool valid =
+            (cur.tile + i) * kTile + tok < cur.ctx && ((masks[s] >> (tok / kBlk)) & 1) != 0;
+        const float ks = scales[s * 2 * kTileBlocks + tok / kBlk];
+        const float vs = valid ? scales[s * 2 * kTileBlocks + kTileBlocks + tok / kBlk] : 1.f;
+        const bool vzero = vs == 0.f;
+        const float lv = vzero ? 0.f : __log2f(vs);
+        const float vinv = vzero ? 1.f : __fdividef(1.f, vs);
+        float x[N];
+#pragma unroll
+        for (int c = 0; c < N; c += 16) tmem_ld16(trow + par * N + c, &x[c]);
+        tmem_wait_ld();
+        float* tops = smax + par * 4 * L::kMaxHeads;
+#pragma unroll
+        for (int h = 0; h < HG; ++h) {
+          const float r = join_terms<kT, HG>(x, h);
+          x[h] = valid ? fmaf(r, qsc[h] * ks, lv) : -INFINITY;
+          const float w = warp_max(x[h]);
+          if (lane == 0) tops[warp * L::kMaxHeads + h] = w;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&top[par]));
+        // The last tile's O, while the other warps' maxima come in.  After it
+        // P and O are free: this tile's PV may write them.
+        if (i > 0) {
+          add_o(j - 1);
+          if (!ok) break;
+        }
+        ok = wait_bar(&top[par], (uint32_t)(j >> 1) & 1u, a.wait_limit_ns);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+#pragma unroll
+        for (int h = 0; h < HG; ++h) {
+          const float mx = fmaxf(fmaxf(tops[h], tops[L::kMaxHeads + h]),
+                                 fmaxf(tops[2 * L::kMaxHeads + h], tops[3 * L::kMaxHeads + h]));
+          const float mn = fmaxf(m[h], mx);
+          const float mu = mn == -INFINITY ? 0.f : mn;
+          alpha[h] = ex2_approx(m[h] - mu);
+          m[h] = mn;
+          x[h] = ex2_approx(x[h] - mu);
+          l[h] = fmaf(l[h], alpha[h], x[h] * vinv);
+        }
+        // P's bytes: column t HG + h is term t of head h
+        uint16_t pairs[N / 2];
+#pragma unroll
+        for (int k = 0; k < N / 2; ++k) pairs[k] = 0;
+        const float ps = vzero ? 0.f : kPScale;
+#pragma unroll
+        for (int h = 0; h < HG; h += 2) {
+          uint16_t t[kT];
+          split_terms<kT>(__floats2half2_rn(x[h] * ps, h + 1 < HG ? x[h + 1 < HG ? h + 1 : h] * ps : 0.f), t);
+#pragma unroll
+          for (int k = 0; k < kT; ++k) {
+            const int c = k * HG + h;
+            if (HG % 2 == 0)
+              pairs[c / 2] = t[k];
+            else  // one head: terms in neighbouring columns
+              pairs[c / 2] |= (uint16_t)((t[k] & 0xffu) << (8 * (c & 1)));
+          }
+        }
+        uint4* pb = reinterpret_cast<uint4*>(smem + L::kPOff) + tok;
+#pragma unroll
+        for (int c = 0; c < N / 16; ++c) {
+          uint32_t w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            w[k] = (uint32_t)pairs[c * 8 + 2 * k] | ((uint32_t)pairs[c * 8 + 2 * k + 1] << 16);
+          pb[c * kTile] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        if (!valid) {
+          // A V row that no token of the row owns (past the context, or a
+          // rejected block's) may hold any bytes, and 0 * NaN is not 0.
+          uint8_t* v = smem + L::kVOff + s * L::kHalf + tok * 128;
+#pragma unroll
+          for (int b = 0; b < L::kBoxes; ++b)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) reinterpret_cast<uint4*>(v + b * kBox)[c] = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        mbar_arrive(smem_addr(p_full));
+      }
+      if (!ok) break;
+      add_o(j - 1);
+
+      // The segment's sums over its 128 token threads, then its result.
+#pragma unroll
+      for (int h = 0; h < HG; ++h) {
+        float w = l[h];
+#pragma unroll
+        for (int k = 16; k > 0; k >>= 1) w += shfl_xor(w, k);
+        if (lane == 0) ssum[warp * L::kMaxHeads + h] = w;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_addr(sums));
+      ok = wait_bar(sums, (uint32_t)seg & 1u, a.wait_limit_ns);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
       }
-      float alpha_new[HG];
-#pragma unroll
-      for (int h = 0; h < HG; ++h) {
-        const float mx = fmaxf(fmaxf(tops[h], tops[L::kMaxHeads + h]),
-                               fmaxf(tops[2 * L::kMaxHeads + h], tops[3 * L::kMaxHeads + h]));
-        const float mn = fmaxf(m[h], mx);
-        const float mu = mn == -INFINITY ? 0.f : mn;
-        alpha_new[h] = ex2_approx(m[h] - mu);
-        m[h] = mn;
-        x[h] = ex2_approx(x[h] - mu);
-        l[h] = fmaf(l[h], alpha_new[h], x[h] * vinv);
-      }
-      // P's bytes: column t HG + h is term t of head h
-      uint16_t pairs[N / 2];
-#pragma unroll
-      for (int i = 0; i < N / 2; ++i) pairs[i] = 0;
-      const float ps = vzero ? 0.f : kPScale;
-#pragma unroll
-      for (int h = 0; h < HG; h += 2) {
-        uint16_t t[kT];
-        split_terms<kT>(__floats2half2_rn(x[h] * ps, h + 1 < HG ? x[h + 1 < HG ? h + 1 : h] * ps : 0.f), t);
-#pragma unroll
-        for (int k = 0; k < kT; ++k) {
-          const int c = k * HG + h;
-          if (HG % 2 == 0)
-            pairs[c / 2] = t[k];
-          else  // one head: terms in neighbouring columns
-            pairs[c / 2] |= (uint16_t)((t[k] & 0xffu) << (8 * (c & 1)));
-        }
-      }
-      uint4* pb = reinterpret_cast<uint4*>(smem + L::kPOff + (j & 1) * L::kPBytes) + tok;
-#pragma unroll
-      for (int c = 0; c < N / 16; ++c) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          w[i] = (uint32_t)pairs[c * 8 + 2 * i] | ((uint32_t)pairs[c * 8 + 2 * i + 1] << 16);
-        pb[c * kTile] = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-      if (!valid) {
-        // A V row that no token of the row owns (past the context, or a
-        // rejected block's) may hold any bytes, and 0 * NaN is not 0.
-        mbar_wait_bounded(smem_addr(&v_full[j % S]), (uint32_t)(j / S) & 1u, a.wait_limit_ns);
-        uint8_t* v = smem + L::kVOff + (j % S) * L::kHalf + tok * 128;
-#pragma unroll
-        for (int b = 0; b < L::kBoxes; ++b)
-#pragma unroll
-          for (int c = 0; c < 8; ++c) reinterpret_cast<uint4*>(v + b * kBox)[c] = make_uint4(0, 0, 0, 0);
-      }
-      fence_proxy_async_smem();
-      tc_fence_before();
-      mbar_arrive(smem_addr(&p_full[j & 1]));
-      if (j > 0) {
-        add_o(j - 1);
-        if (!ok) break;
-      }
-#pragma unroll
-      for (int h = 0; h < HG; ++h) alpha[h] = alpha_new[h];
-      id_cur = id_nxt;
-      id_nxt = id_nn;
-      ks = ks_nxt;
-      vs = vs_nxt;
-    }
-    if (ok && ntiles > 0) add_o(ntiles - 1);
-    if (!ok && lane == 0) block_attn_error(CF_DEVERR_TIMEOUT);
-
-    // The row's sums over its 128 token threads, then this thread's dimension.
-#pragma unroll
-    for (int h = 0; h < HG; ++h) {
-      float w = l[h];
-      for (int i = 16; i > 0; i >>= 1) w += shfl_xor(w, i);
-      if (lane == 0) ssum[warp * L::kMaxHeads + h] = w;
-    }
-    if (lane == 0) sok[warp] = ok ? 1 : 0;
-    asm volatile("bar.sync 1, 128;" ::: "memory");  // every softmax warp comes here, with or without a timeout
-    if (sok[0] & sok[1] & sok[2] & sok[3]) {  // after a timeout nothing is written
+      const bool whole = cur.tile == 0 && cnt == cur.tiles;
+      const int slot = 2 * blockIdx.x + (cur.tile == 0 ? 1 : 0);
+      const int head0 = kvh * a.group + chunk * HG, nheads = min(HG, a.group - chunk * HG);
 #pragma unroll
       for (int h = 0; h < HG; ++h) {
         if (h >= nheads) continue;
         const float sum = (ssum[h] + ssum[L::kMaxHeads + h]) + (ssum[2 * L::kMaxHeads + h] + ssum[3 * L::kMaxHeads + h]);
-        const size_t hq = (size_t)seq * a.num_heads + head0 + h;
         const float inv = sum == 0.f ? 0.f : 1.f / (sum * kPScale);
 #pragma unroll
         for (int b = 0; b < L::kBoxes; ++b) {
           const float r = acc[b][h] * inv;
-          if (single)
-            static_cast<T*>(a.out)[hq * D + b * 128 + tok] = from_float<T>(r);
+          if (whole)
+            static_cast<T*>(a.out)[((size_t)cur.seq * a.num_heads + head0 + h) * D + b * 128 + tok] = from_float<T>(r);
           else
-            a.part_out[(hq * a.num_parts + part) * D + b * 128 + tok] = r;
+            a.part_out[((size_t)slot * HG + h) * D + b * 128 + tok] = r;
         }
-        if (!single && tok == 0) {
-          a.part_max[hq * a.num_parts + part] = m[h];
-          a.part_sum[hq * a.num_parts + part] = sum;
+        if (!whole && tok == 0) {
+          a.part_max[slot * HG + h] = m[h];
+          a.part_sum[slot * HG + h] = sum;
         }
       }
+      if (!whole && cur.tile == 0 && tok == 0) {
+        // an item begun here and finished by the CTA that has its last tile
+        const int64_t* scan = reinterpret_cast<const int64_t*>(smem + L::kScanOff);
+        const int64_t last = scan[0] + (j - cnt) + cur.tiles - 1;
+        a.meta[blockIdx.x] = make_int4(cur.seq, cur.item, (int)(((last + 1) * scan[3] - 1) / scan[2]), 0);
+        begun = true;
+      }
     }
+    if (!ok && lane == 0) block_attn_error(CF_DEVERR_TIMEOUT);
+    if (a.meta != nullptr && tok == 0 && !begun) a.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
   }
   grid_dependency_launch();
   tc_fence_before();
@@ -618,40 +803,82 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
   if (warp == kMmaWarp) tmem_dealloc(tmem, L::kTmemCols);
 }
 
-// Merges a row's partitions, one warp per (query head, row):
+// Joins the items that several CTAs share, one CTA of D threads per (CTA of
+// the streaming kernel, head): the item that CTA c began, its later pieces in
+// the first slots of CTAs c + 1 .. last.
 // out = sum_p w_p o_p / sum_p w_p, w_p = sum_p 2^(max_p - max).
-template <typename T, int D>
-__global__ void __launch_bounds__(128) block_attention_merge_kernel(const Args a) {
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int head = blockIdx.x * 4 + (threadIdx.x >> 5), seq = blockIdx.y;
-  if (head >= a.num_heads) return;
+template <typename T, int D, int HG>
+__global__ void __launch_bounds__(D) block_attention_join_kernel(const Args a) {
+  extern __shared__ float w_sh[];  // a weight per piece
+  __shared__ float red[2][D / 32];
   grid_dependency_wait();
-  const int ctx = context_of(a, seq, false);
-  const int parts = min(a.num_parts, (ctx + a.part_tokens - 1) / a.part_tokens);
-  if (parts <= 1) return;  // written by the partition kernel
-  const size_t base = ((size_t)seq * a.num_heads + head) * a.num_parts;
+  const int c = blockIdx.x, h = blockIdx.y;
+  const int4 meta = a.meta[c];
+  if (meta.x < 0) return;
+  const int kvh = meta.y / a.head_chunks, chunk = meta.y - kvh * a.head_chunks;
+  if (h >= min(HG, a.group - chunk * HG)) return;
+  const int pieces = meta.z - c + 1;
+  auto slot = [&](int p) { return (size_t)(p == 0 ? 2 * c + 1 : 2 * (c + p)) * HG + h; };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float m = -INFINITY;
-  for (int p = lane; p < parts; p += 32) m = fmaxf(m, a.part_max[base + p]);
+  for (int p = threadIdx.x; p < pieces; p += D) m = fmaxf(m, a.part_max[slot(p)]);
+#pragma unroll
   for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, shfl_xor(m, i));
-  float l = 0.f, o[E];
+  if (lane == 0) red[0][warp] = m;
+  __syncthreads();
 #pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.f;
-  if (m != -INFINITY) {
-#pragma unroll 4
-    for (int p = 0; p < parts; ++p) {
-      const float w = a.part_sum[base + p] * exp2f(a.part_max[base + p] - m);
-      l += w;
-      float x[E];
-      load_widen<float, E>(a.part_out + (base + p) * D + lane * E, x);
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = fmaf(w, x[e], o[e]);
-    }
+  for (int i = 0; i < D / 32; ++i) m = fmaxf(m, red[0][i]);
+  float l = 0.f;
+  for (int p = threadIdx.x; p < pieces; p += D) {
+    const float sum = a.part_sum[slot(p)];
+    // a piece without a readable token has sum 0 and max -inf
+    const float w = sum == 0.f ? 0.f : sum * exp2f(a.part_max[slot(p)] - m);
+    w_sh[p] = w;
+    l += w;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  T* out = static_cast<T*>(a.out) + ((size_t)seq * a.num_heads + head) * D + lane * E;
 #pragma unroll
-  for (int e = 0; e < E; ++e) out[e] = from_float<T>(o[e] * inv);
+  for (int i = 16; i > 0; i >>= 1) l += shfl_xor(l, i);
+  if (lane == 0) red[1][warp] = l;
+  __syncthreads();
+  l = 0.f;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) l += red[1][i];
+  float o = 0.f;
+#pragma unroll 8
+  for (int p = 0; p < pieces; ++p) o = fmaf(w_sh[p], a.part_out[slot(p) * D + threadIdx.x], o);
+  const int head = kvh * a.group + chunk * HG + h;
+  static_cast<T*>(a.out)[((size_t)meta.x * a.num_heads + head) * D + threadIdx.x] =
+      from_float<T>(l == 0.f ? 0.f : o / l);
+}
+
+// ---------------------------------------------------------------------------
+// Host side.
+// ---------------------------------------------------------------------------
+// Streaming CTAs that are resident at once on the current device.
+template <typename T, int D, int HG>
+int resident_ctas() {
+  int dev = 0, n = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess)
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  else
+    cudaGetLastError();
+  return (n > 0 ? n : 148) * Layout<T, D, HG>::kMinCtas;
+}
+
+struct Workspace {
+  size_t meta, max, sum, out, bytes;
+};
+
+Workspace workspace_of(int ctas, int hg, int d) {
+  auto round = [](size_t b) { return (b + 255) / 256 * 256; };
+  const size_t rows = (size_t)2 * ctas * hg;
+  Workspace w;
+  w.meta = 0;
+  w.max = round((size_t)ctas * sizeof(int4));
+  w.sum = w.max + round(rows * 4);
+  w.out = w.sum + round(rows * 4);
+  w.bytes = w.out + round(rows * d * 4);
+  return w;
 }
 
 // Per kernel instantiation and device: opt in to > 48 KB of dynamic smem.
@@ -659,23 +886,29 @@ template <typename T, int D, int HG>
 cf_status ensure_smem() {
   static std::once_flag flags[64];
   static cudaError_t errs[64];
-  auto kern = block_attention_kernel<T, D, HG>;
-  constexpr int bytes = Layout<T, D, HG>::kAlloc;
+  auto set = [] {
+    auto kern = block_attention_kernel<T, D, HG>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<T, D, HG>::kAlloc);
+    if (Layout<T, D, HG>::kSplitRegs && e == cudaSuccess) {
+      // a build with fewer registers than the split shares out must not run
+      cudaFuncAttributes fa;
+      e = cudaFuncGetAttributes(&fa, kern);
+      if (e == cudaSuccess && fa.numRegs < Layout<T, D, HG>::kLaunchRegs) e = cudaErrorInvalidConfiguration;
+    }
+    return e;
+  };
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_status(e);
-  if (dev < 0 || dev >= 64)
-    return cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  std::call_once(flags[dev], [&] {
-    errs[dev] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  });
+  if (dev < 0 || dev >= 64) return cuda_status(set());
+  std::call_once(flags[dev], [&] { errs[dev] = set(); });
   return cuda_status(errs[dev]);
 }
 
 template <typename T, int D, int HG>
-cf_status launch_heads(Args a, const cf_paged_attention_params& p, cudaStream_t stream) {
+cf_status launch_heads(Args a, const BlockScaledLaunch& l) {
+  const cf_paged_attention_params& p = *l.p;
   a.head_chunks = (a.group + HG - 1) / HG;
-  if ((int64_t)p.num_kv_heads * a.head_chunks > 65535) return CF_ERR_UNSUPPORTED;
   CUtensorMap mk, mv;
   const int64_t rows = p.num_blocks * (int64_t)p.num_kv_heads * kBlk;
   if (!kv_tensor_map(&mk, p.key_cache, rows, D, CF_FP8_E4M3) ||
@@ -683,36 +916,76 @@ cf_status launch_heads(Args a, const cf_paged_attention_params& p, cudaStream_t 
     return CF_ERR_CUDA;
   cf_status st = ensure_smem<T, D, HG>();
   if (st != CF_OK) return st;
-  const dim3 grid((unsigned)a.num_parts, (unsigned)(p.num_kv_heads * a.head_chunks), (unsigned)p.num_seqs);
-  block_attention_kernel<T, D, HG><<<grid, kThreads, Layout<T, D, HG>::kAlloc, stream>>>(a, mk, mv);
-  return check_launch();
-}
-
-template <typename T, int D>
-cf_status launch_dim(const Args& a, const cf_paged_attention_params& p, cudaStream_t stream) {
-  cf_status st;
-  if (a.group == 1)
-    st = launch_heads<T, D, 1>(a, p, stream);
-  else if (a.group <= 4)
-    st = launch_heads<T, D, 4>(a, p, stream);
-  else if (a.group <= 8)
-    st = launch_heads<T, D, 8>(a, p, stream);
-  else
-    st = launch_heads<T, D, 16>(a, p, stream);
-  if (st != CF_OK || a.part_max == nullptr) return st;
+  const int ctas = resident_ctas<T, D, HG>();
+  const int64_t items = (int64_t)p.num_seqs * p.num_kv_heads * a.head_chunks;
+  const int64_t tiles = p.max_context_len > kTile ? (p.max_context_len + kTile - 1) / kTile : 1;
+  const Workspace w = workspace_of(ctas, HG, D);
+  const bool share = tiles > 1 && l.workspace != nullptr && l.workspace_bytes >= w.bytes;
+  if (share) {
+    uint8_t* base = static_cast<uint8_t*>(l.workspace);
+    a.meta = reinterpret_cast<int4*>(base + w.meta);
+    a.part_max = reinterpret_cast<float*>(base + w.max);
+    a.part_sum = reinterpret_cast<float*>(base + w.sum);
+    a.part_out = reinterpret_cast<float*>(base + w.out);
+  }
+  const int64_t want = share ? items * tiles : items;
+  const unsigned grid = (unsigned)(want < ctas ? want : ctas);
+  block_attention_kernel<T, D, HG><<<grid, kThreads, Layout<T, D, HG>::kAlloc, l.stream>>>(a, mk, mv);
+  st = check_launch();
+  if (st != CF_OK || !share) return st;
   cudaLaunchConfig_t cfg = {};
-  cfg.stream = stream;
+  cfg.stream = l.stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cfg.gridDim = dim3((unsigned)((a.num_heads + 3) / 4), (unsigned)p.num_seqs);
-  cfg.blockDim = dim3(128);
-  return cuda_status(cudaLaunchKernelEx(&cfg, block_attention_merge_kernel<T, D>, a));
+  cfg.gridDim = dim3(grid, (unsigned)(a.group < HG ? a.group : HG));
+  cfg.blockDim = dim3(D);
+  cfg.dynamicSmemBytes = grid * sizeof(float);
+  return cuda_status(cudaLaunchKernelEx(&cfg, block_attention_join_kernel<T, D, HG>, a));
 }
 
+// Calls f with the kernel's types as template arguments: HG query heads of a
+// KV head per item.
+template <typename F>
+auto dispatch(const cf_paged_attention_params& p, F&& f) {
+  const int group = p.num_heads / p.num_kv_heads;
+  auto heads = [&](auto t, auto d) {
+    using Tp = decltype(t);
+    constexpr int D = decltype(d)::value;
+    if (group == 1) return f.template operator()<Tp, D, 1>();
+    if (group <= 4) return f.template operator()<Tp, D, 4>();
+    if (group <= 8) return f.template operator()<Tp, D, 8>();
+    return f.template operator()<Tp, D, 16>();
+  };
+  using D128 = std::integral_constant<int, 128>;
+  using D256 = std::integral_constant<int, 256>;
+  if (p.dtype == CF_F16) return p.head_dim == 128 ? heads(__half{}, D128{}) : heads(__half{}, D256{});
+  return p.head_dim == 128 ? heads(__nv_bfloat16{}, D128{}) : heads(__nv_bfloat16{}, D256{});
+}
+
+struct SizeOf {
+  template <typename T, int D, int HG>
+  size_t operator()() const {
+    return workspace_of(resident_ctas<T, D, HG>(), HG, D).bytes;
+  }
+};
+
+struct Launch {
+  const Args& a;
+  const BlockScaledLaunch& l;
+  template <typename T, int D, int HG>
+  cf_status operator()() const {
+    return launch_heads<T, D, HG>(a, l);
+  }
+};
+
 }  // namespace
+
+size_t block_scaled_workspace(const cf_paged_attention_params& p) {
+  return p.num_seqs > 0 && p.max_context_len > kTile ? dispatch(p, SizeOf{}) : 0;
+}
 
 cf_status launch_block_scaled_attention(const BlockScaledLaunch& l) {
   const cf_paged_attention_params& p = *l.p;
@@ -724,28 +997,17 @@ cf_status launch_block_scaled_attention(const BlockScaledLaunch& l) {
   a.tables = p.block_tables;
   a.lens = p.context_lens;
   a.scale_log2 = p.scale * kLog2e;
+  a.num_seqs = p.num_seqs;
   a.num_heads = p.num_heads;
   a.num_kv_heads = p.num_kv_heads;
   a.group = p.num_heads / p.num_kv_heads;
   a.max_blocks = p.max_blocks_per_seq;
-  a.num_parts = l.num_parts;
-  // unsplit: one partition, whole tiles
-  a.part_tokens = l.num_parts > 1 ? l.part_tokens : (p.max_blocks_per_seq * kBlk + kTile - 1) / kTile * kTile;
   a.num_blocks = p.num_blocks;
   const int64_t lim = g_test_wait_limit_ns.load(std::memory_order_relaxed);
   a.wait_limit_ns = lim > 0 ? (uint64_t)lim : kWaitLimitNs;
   a.unarm_first_stage = g_test_unarm_first_stage.load(std::memory_order_relaxed);
-  if (l.num_parts > 1) {
-    a.part_max = l.part_max;
-    a.part_sum = l.part_sum;
-    a.part_out = l.part_out;
-  }
-  if (p.dtype == CF_F16)
-    return p.head_dim == 128 ? launch_dim<__half, 128>(a, p, l.stream) : launch_dim<__half, 256>(a, p, l.stream);
-  return p.head_dim == 128 ? launch_dim<__nv_bfloat16, 128>(a, p, l.stream)
-                           : launch_dim<__nv_bfloat16, 256>(a, p, l.stream);
+  return dispatch(p, Launch{a, l});
 }
-
 cf_status block_scaled_read_errors(uint32_t* bits, bool clear) {
   uint32_t v = 0;
   cf_status s = cuda_status(cudaMemcpyFromSymbol(&v, g_block_attn_errors, sizeof(v)));

@@ -248,23 +248,6 @@ cf_status check_block_cache(int32_t head_dim, int32_t block_size, int64_t num_bl
   return CF_OK;
 }
 
-// Split of the block-scaled decode attention: partitions and their tokens, and
-// the workspace they take (0: unsplit).
-size_t block_split(const cf_paged_attention_params* p, int32_t* parts_out, int32_t* tokens_out) {
-  if (p->num_seqs <= 0) return 0;
-  constexpr int64_t kTargetCtas = 4 * 148;
-  const int64_t pairs = (int64_t)p->num_seqs * p->num_kv_heads;
-  int32_t split = 2048;
-  while (split > 128 && pairs * ((p->max_context_len + split - 1) / split) < kTargetCtas) split /= 2;
-  if (p->max_context_len <= split) return 0;
-  const int64_t parts = ((int64_t)p->max_context_len + split - 1) / split;
-  if (parts_out) *parts_out = (int32_t)parts;
-  if (tokens_out) *tokens_out = split;
-  const int64_t rows = (int64_t)p->num_seqs * p->num_heads * parts;
-  auto round = [](int64_t b) { return (b + 255) / 256 * 256; };
-  return (size_t)(2 * round(rows * 4) + round(rows * p->head_dim * 4));
-}
-
 }  // namespace
 }  // namespace cfb
 
@@ -555,16 +538,7 @@ cf_status cf_reshape_and_cache_fp8_block(const void* key, const void* value, voi
 size_t cf_paged_attention_fp8_block_workspace_size(const cf_paged_attention_params* p) {
   if (check_attention_params(p, /*check_pointers=*/false) != CF_OK) return 0;
   if (check_fp8(p, 1.f, 1.f) != CF_OK || p->num_blocks <= 0) return 0;
-  // the most that any max_context_len up to this one takes
-  cf_paged_attention_params q = *p;
-  size_t bytes = 0;
-  for (int64_t c = 128;; c += 128) {
-    q.max_context_len = (int32_t)(c < p->max_context_len ? c : p->max_context_len);
-    const size_t b = block_split(&q, nullptr, nullptr);
-    bytes = b > bytes ? b : bytes;
-    if (c >= p->max_context_len) break;
-  }
-  return bytes;
+  return block_scaled_workspace(*p);
 }
 
 cf_status cf_paged_attention_fp8_block_v1(const cf_paged_attention_params* p, const float* k_scales,
@@ -577,20 +551,8 @@ cf_status cf_paged_attention_fp8_block_v1(const cf_paged_attention_params* p, co
   // TMA rows and token counts are int32
   if (p->num_blocks > INT32_MAX / p->block_size / p->num_kv_heads || p->max_blocks_per_seq > (INT32_MAX - 128) / 16)
     return CF_ERR_UNSUPPORTED;
-  BlockScaledLaunch l{p, k_scales, v_scales, 0, 1, nullptr, nullptr, nullptr, (cudaStream_t)stream};
-  int32_t parts = 1, tokens = 0;
-  const size_t need = block_split(p, &parts, &tokens);
-  if (need > 0 && workspace != nullptr && workspace_bytes >= need) {
-    if (!aligned16(workspace)) return CF_ERR_INVALID_ARGUMENT;
-    const int64_t r4 = ((int64_t)p->num_seqs * p->num_heads * parts * 4 + 255) / 256 * 256;
-    uint8_t* w = static_cast<uint8_t*>(workspace);
-    l.part_tokens = tokens;
-    l.num_parts = parts;
-    l.part_max = reinterpret_cast<float*>(w);
-    l.part_sum = reinterpret_cast<float*>(w + r4);
-    l.part_out = reinterpret_cast<float*>(w + 2 * r4);
-  }
-  return launch_block_scaled_attention(l);
+  if (workspace != nullptr && !aligned16(workspace)) return CF_ERR_INVALID_ARGUMENT;
+  return launch_block_scaled_attention({p, k_scales, v_scales, workspace, workspace_bytes, (cudaStream_t)stream});
 }
 
 cf_status cf_copy_blocks(void* key_cache, void* value_cache, const int64_t* block_mapping,

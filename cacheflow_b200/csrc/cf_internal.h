@@ -115,13 +115,13 @@ struct BlockScaledLaunch {
   const cf_paged_attention_params* p;
   const float* k_scales;
   const float* v_scales;
-  int32_t part_tokens;  // tokens per partition (num_parts > 1)
-  int32_t num_parts;    // 1: unsplit
-  float* part_max;      // [num_seqs, num_heads, num_parts]
-  float* part_sum;
-  float* part_out;      // [num_seqs, num_heads, num_parts, head_dim]
+  void* workspace;  // null, or block_scaled_workspace() bytes
+  size_t workspace_bytes;
   cudaStream_t stream;
 };
+// Workspace of any call with these heads and head_dim on the current device;
+// 0 where no context needs sharing.
+size_t block_scaled_workspace(const cf_paged_attention_params& p);
 cf_status launch_block_scaled_attention(const BlockScaledLaunch& l);
 cf_status block_scaled_read_errors(uint32_t* bits, bool clear);
 
