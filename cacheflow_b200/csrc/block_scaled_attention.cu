@@ -150,12 +150,13 @@ struct Layout {
   static constexpr int kQBox = kN * 128;
   static constexpr int kPOff = kQOff + kBoxes * kQBox;  // P: kN/16 planes x 128 tokens x 16 B
   static constexpr int kBarOff = kPOff + kN * 128;
-  // full, empty of K and of V; s_full and top by tile parity; p_full, o_full,
-  // q_full, q_empty, sums, fin
-  static constexpr int kNumBars = 4 * kStages + 2 * 2 + 6;
+  // full, empty of K and of V; s_full by tile parity; p_full, o_full, q_full,
+  // q_empty, fin
+  static constexpr int kNumBars = 4 * kStages + 2 + 5;
   static constexpr int kScaleOff = kBarOff + (kNumBars * 8 + 15) / 16 * 16;  // [stages][ks 8, vs 8] f32
   static constexpr int kMaskOff = kScaleOff + kStages * 2 * kTileBlocks * 4;  // [stages] int
-  static constexpr int kMaxOff = kMaskOff + 16;                               // [2][4][HG] f32
+  static constexpr int kFailOff = kMaskOff + 16;                              // int: a wait ran out
+  static constexpr int kMaxOff = kFailOff + 16;                               // [2][4][HG] f32
   static constexpr int kMaxHeads = (HG + 3) / 4 * 4;
   static constexpr int kSumOff = kMaxOff + 2 * 4 * kMaxHeads * 4;          // [4][HG] f32
   static constexpr int kQsOff = kSumOff + 4 * kMaxHeads * 4;               // [HG] f32
@@ -204,24 +205,21 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// mbar_wait_bounded with the barrier unit asked to hold the thread for up to
-// 2 us per try: warps that wait for another role leave the issue slots to it.
+// Waits for phase `parity` of *bar, at most limit_ns (false then).  Roles with
+// time to spare sleep kSleep ns between their tries and leave the issue slots
+// to the softmax.
+template <int kSleep = 0>
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
   const uint32_t b = smem_addr(bar);
-  uint64_t t0 = 0;
+  if (mbar_try_wait(b, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
   while (true) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(b), "r"(parity), "r"(2000u)
-        : "memory");
-    if (ok) return true;
-    const uint64_t t = global_timer_ns();
-    if (t0 == 0) t0 = t;
-    if (t - t0 > limit_ns) return false;
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i) {
+      if (kSleep > 0) __nanosleep(kSleep);
+      if (mbar_try_wait(b, parity)) return true;
+    }
+    if (global_timer_ns() - t0 > limit_ns) return false;
   }
 }
 
@@ -346,16 +344,15 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
   uint64_t* k_empty = bars + S;
   uint64_t* v_full = bars + 2 * S;
   uint64_t* v_empty = bars + 3 * S;
-  uint64_t* s_full = bars + 4 * S;  // [2], by tile parity, as top
-  uint64_t* top = s_full + 2;
-  uint64_t* p_full = top + 2;
+  uint64_t* s_full = bars + 4 * S;  // [2], by tile parity
+  uint64_t* p_full = s_full + 2;
   uint64_t* o_full = p_full + 1;
   uint64_t* q_full = o_full + 1;
   uint64_t* q_empty = q_full + 1;
-  uint64_t* sums = q_empty + 1;
-  uint64_t* fin = sums + 1;
+  uint64_t* fin = q_empty + 1;
   float* scales = reinterpret_cast<float*>(smem + L::kScaleOff);
   int* masks = reinterpret_cast<int*>(smem + L::kMaskOff);
+  volatile int* fail = reinterpret_cast<int*>(smem + L::kFailOff);  // of a softmax warp
   float* smax = reinterpret_cast<float*>(smem + L::kMaxOff);
   float* ssum = reinterpret_cast<float*>(smem + L::kSumOff);
   float* sqs = reinterpret_cast<float*>(smem + L::kQsOff);
@@ -368,16 +365,13 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
       mbar_init(smem_addr(&v_full[s]), 1 + 2 * kTileBlocks);  // V's bytes, and 16 lanes' scales
       mbar_init(smem_addr(&v_empty[s]), 1);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_addr(&s_full[i]), 1);
-      mbar_init(smem_addr(&top[i]), 4);
-    }
+    for (int i = 0; i < 2; ++i) mbar_init(smem_addr(&s_full[i]), 1);
     mbar_init(smem_addr(p_full), kTile);
     mbar_init(smem_addr(o_full), 1);
     mbar_init(smem_addr(q_full), 32);
     mbar_init(smem_addr(q_empty), 1 + 4);  // its last QK, and the softmax warps' reads of the scales
-    mbar_init(smem_addr(sums), 4);
     mbar_init(smem_addr(fin), 1);
+    *fail = 0;
     fence_mbar_init();
   }
   if (warp == kMmaWarp) {
@@ -388,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
   Cursor cur = find_start<L>(a, smem);  // synchronises the block
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int64_t ntiles = cur.left;  // of this CTA
+  const uint32_t ntiles = (uint32_t)cur.left;  // of this CTA (its share of all tiles is far below 2^31)
 
   // Rows without a context: zeros, dealt to the CTAs in turn.
   for (int s = blockIdx.x; s < a.num_seqs; s += gridDim.x)
@@ -407,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
       uint8_t* ring = smem + (is_k ? 0 : L::kVOff);
       const CUtensorMap* map = is_k ? &tmk : &tmv;
       bool ok = true;
-      int64_t j = 0;  // tiles begun
+      uint32_t j = 0;  // tiles begun
       // Block ids come 32 (four tiles) at a time, a group ahead of their use:
       // `ahead` stands at the group whose ids are in `ids_next`.
       Cursor ahead = cur;
@@ -444,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
           if (want && !valid && lane < kTileBlocks) block_attn_error(CF_DEVERR_BLOCK_ID);
           const uint32_t mask = __ballot_sync(0xffffffffu, valid) & 0xffu;
           if (j >= S) {
-            ok = wait_bar(&empties[s], (uint32_t)(j / S - 1) & 1u, a.wait_limit_ns);
+            ok = wait_bar<64>(&empties[s], (j / S - 1) & 1u, a.wait_limit_ns);
             if (!__all_sync(0xffffffffu, ok)) {
               ok = false;
               break;
@@ -480,8 +474,7 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
       // no copy may land after the CTA has left
       cp_async_wait_all();
       if (lane == 0)
-        for (int64_t i = j > S ? j - S : 0; i < j; ++i)
-          wait_bar(&fulls[i % S], (uint32_t)(i / S) & 1u, a.wait_limit_ns);
+        for (uint32_t i = j > S ? j - S : 0; i < j; ++i) wait_bar(&fulls[i % S], (i / S) & 1u, a.wait_limit_ns);
     } else if (warp == kQWarp) {
       // ---------------- Q's terms, a segment at a time ----------------
       constexpr int E = D / 32;
@@ -503,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
             for (int e = 0; e < E / 2; ++e)
               raw[h][e] = h0 + h < nheads ? reinterpret_cast<const uint32_t*>(src + (size_t)(h0 + h) * D)[e] : 0u;
           if (h0 == 0 && seg > 0) {
-            ok = wait_bar(q_empty, (uint32_t)(seg - 1) & 1u, a.wait_limit_ns);
+            ok = wait_bar<256>(q_empty, (uint32_t)(seg - 1) & 1u, a.wait_limit_ns);
             if (!__all_sync(0xffffffffu, ok)) {
               ok = false;
               break;
@@ -562,10 +555,10 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
       const uint64_t p_desc = smem_desc_plain(smem_addr(smem + L::kPOff), 128, kTile * 16);
       bool ok = true;
       int seg = 0, i = 0;  // segment and its next tile, of the next QK
-      auto issue_qk = [&](int64_t j) {
+      auto issue_qk = [&](uint32_t j) {
         const int s = (int)(j % S);
-        ok = ok && (i > 0 || wait_bar(q_full, (uint32_t)seg & 1u, a.wait_limit_ns)) &&
-             wait_bar(&k_full[s], (uint32_t)(j / S) & 1u, a.wait_limit_ns);
+        ok = ok && (i > 0 || wait_bar<32>(q_full, (uint32_t)seg & 1u, a.wait_limit_ns)) &&
+             wait_bar<32>(&k_full[s], (j / S) & 1u, a.wait_limit_ns);
         if (!ok) return;
         tc_fence_after();
         const uint64_t kd = k_desc + (uint64_t)((s * L::kHalf) >> 4);
@@ -584,11 +577,11 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
           cur.next(a);
         }
       };
-      for (int64_t j = 0; j < 2 && j < ntiles; ++j) issue_qk(j);
-      for (int64_t j = 0; j < ntiles && ok; ++j) {
+      for (uint32_t j = 0; j < 2 && j < ntiles; ++j) issue_qk(j);
+      for (uint32_t j = 0; j < ntiles && ok; ++j) {
         const int s = (int)(j % S);
-        ok = wait_bar(p_full, (uint32_t)j & 1u, a.wait_limit_ns) &&
-             wait_bar(&v_full[s], (uint32_t)(j / S) & 1u, a.wait_limit_ns);
+        ok = wait_bar<32>(p_full, (uint32_t)j & 1u, a.wait_limit_ns) &&
+             wait_bar<32>(&v_full[s], (j / S) & 1u, a.wait_limit_ns);
         if (!ok) break;
         tc_fence_after();
         const uint64_t vd = v_desc + (uint64_t)((s * L::kHalf) >> 4);
@@ -615,17 +608,24 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
     if constexpr (L::kSplitRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kSoftmaxRegs));
     const int tok = threadIdx.x;  // token of the tile; head dimension of O
     const uint32_t trow = tmem + ((uint32_t)(32 * warp) << 16);
-    bool ok = true, begun = false;
-    int64_t j = 0;
+    bool begun = false;
+    uint32_t j = 0;
+    // Warp 0 waits for the others, which sleep at a hardware barrier: polling
+    // warps would take the issue slots of the other CTAs' softmax.  A wait
+    // that runs out sets *fail; every warp sees it after the next barrier and
+    // leaves, so the four warps meet at every barrier.
+    auto meet = [&]() {
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      return *fail == 0;
+    };
+    bool ok = true;
     for (int seg = 0; !cur.done(); cur.next(a), ++seg) {
       const int cnt = cur.count();
       const int kvh = cur.item / a.head_chunks, chunk = cur.item - kvh * a.head_chunks;
       float qsc[HG], m[HG], l[HG], alpha[HG], acc[L::kBoxes][HG];
-      ok = wait_bar(q_full, (uint32_t)seg & 1u, a.wait_limit_ns);
-      if (!__all_sync(0xffffffffu, ok)) {
-        ok = false;
-        break;
-      }
+      if (warp == 0 && !wait_bar(q_full, (uint32_t)seg & 1u, a.wait_limit_ns)) *fail = 1;
+      ok = meet();
+      if (!ok) break;
 #pragma unroll
       for (int h = 0; h < HG; ++h) {
         qsc[h] = sqs[h] * a.scale_log2;
@@ -637,12 +637,9 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_addr(q_empty));
-      auto add_o = [&](int64_t t) {  // the accumulator takes tile t's O
-        ok = wait_bar(o_full, (uint32_t)t & 1u, a.wait_limit_ns);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          return;
-        }
+      auto add_o = [&](uint32_t t) {  // the accumulator takes tile t's O
+        if (!wait_bar(o_full, t & 1u, a.wait_limit_ns)) *fail = 1;
+        __syncwarp();
         tc_fence_after();
 #pragma unroll
         for (int b = 0; b < L::kBoxes; ++b) {
@@ -656,12 +653,11 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
       };
       for (int i = 0; i < cnt; ++i, ++j) {
         const int par = (int)(j & 1), s = (int)(j % S);
-        ok = wait_bar(&v_full[s], (uint32_t)(j / S) & 1u, a.wait_limit_ns) &&
-             wait_bar(&s_full[par], (uint32_t)(j >> 1) & 1u, a.wait_limit_ns);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
+        if (warp == 0 && !(wait_bar(&v_full[s], (j / S) & 1u, a.wait_limit_ns) &&
+                           wait_bar(&s_full[par], (j >> 1) & 1u, a.wait_limit_ns)))
+          *fail = 1;
+        ok = meet();
+        if (!ok) break;
         tc_fence_after();
         const bool valid =
             (cur.tile + i) * kTile + tok < cur.ctx && ((masks[s] >> (tok / kBlk)) & 1) != 0;
@@ -682,19 +678,11 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
           const float w = warp_max(x[h]);
           if (lane == 0) tops[warp * L::kMaxHeads + h] = w;
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_addr(&top[par]));
         // The last tile's O, while the other warps' maxima come in.  After it
         // P and O are free: this tile's PV may write them.
-        if (i > 0) {
-          add_o(j - 1);
-          if (!ok) break;
-        }
-        ok = wait_bar(&top[par], (uint32_t)(j >> 1) & 1u, a.wait_limit_ns);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
+        if (i > 0) add_o(j - 1);
+        ok = meet();
+        if (!ok) break;
 #pragma unroll
         for (int h = 0; h < HG; ++h) {
           const float mx = fmaxf(fmaxf(tops[h], tops[L::kMaxHeads + h]),
@@ -757,13 +745,8 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
         for (int k = 16; k > 0; k >>= 1) w += shfl_xor(w, k);
         if (lane == 0) ssum[warp * L::kMaxHeads + h] = w;
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_addr(sums));
-      ok = wait_bar(sums, (uint32_t)seg & 1u, a.wait_limit_ns);
-      if (!__all_sync(0xffffffffu, ok)) {
-        ok = false;
-        break;
-      }
+      ok = meet();
+      if (!ok) break;
       const bool whole = cur.tile == 0 && cnt == cur.tiles;
       const int slot = 2 * blockIdx.x + (cur.tile == 0 ? 1 : 0);
       const int head0 = kvh * a.group + chunk * HG, nheads = min(HG, a.group - chunk * HG);
@@ -788,7 +771,7 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
       if (!whole && cur.tile == 0 && tok == 0) {
         // an item begun here and finished by the CTA that has its last tile
         const int64_t* scan = reinterpret_cast<const int64_t*>(smem + L::kScanOff);
-        const int64_t last = scan[0] + (j - cnt) + cur.tiles - 1;
+        const int64_t last = scan[0] + (int64_t)(j - cnt) + cur.tiles - 1;
         a.meta[blockIdx.x] = make_int4(cur.seq, cur.item, (int)(((last + 1) * scan[3] - 1) / scan[2]), 0);
         begun = true;
       }
