@@ -27,8 +27,12 @@ constexpr int kBlk = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // One launch's work is the tiles (128 tokens) of every (row, KV head [, head
-// chunk]) item, rows outermost, laid end to end; CTA c of G takes the tiles
-// [c W / G, (c + 1) W / G) of their W, whatever items they belong to.
+// chunk]) item, rows outermost, laid end to end and cut into equal shares, one
+// for each CTA, whatever items they belong to.  Beginning and ending an item
+// costs a CTA about 0.7 tiles' time (1.4 us), so an item counts 3 quarters of
+// a tile beside its tiles where CTAs have many (without it the CTAs of 256
+// rows of 512-8192 tokens that got the short rows ended at 278 us, half of
+// them before 228).
 struct Args {
   const void* q;
   const float* ks;
@@ -53,6 +57,9 @@ struct Args {
 };
 
 constexpr int kTile = 128;                 // tokens of a tile
+constexpr int kTileWeight = 4;             // of a tile in the shares
+constexpr int kItemWeight = 3;             // of an item's beginning and end
+constexpr int kManyTiles = 8;              // per CTA, from which on that counts
 constexpr int kTileBlocks = kTile / kBlk;  // 8
 constexpr int kBox = kTile * 128;          // 128 rows x 128 bytes
 
@@ -72,8 +79,8 @@ struct Cursor {
   int seq, item;  // row; KV head * chunks + chunk
   int ctx, tiles; // of the row
   int tile;       // first tile of the segment
-  int64_t left;   // tiles of the CTA from here on
-  __device__ __forceinline__ int count() const { return (int)(left < tiles - tile ? left : (int64_t)(tiles - tile)); }
+  int left;       // tiles of the CTA from here on
+  __device__ __forceinline__ int count() const { return min(left, tiles - tile); }
   __device__ __forceinline__ bool done() const { return left <= 0; }
   __device__ __forceinline__ void next(const Args& a) {
     left -= count();
@@ -160,9 +167,10 @@ struct Layout {
   static constexpr int kMaxHeads = (HG + 3) / 4 * 4;
   static constexpr int kSumOff = kMaxOff + 2 * 4 * kMaxHeads * 4;          // [4][HG] f32
   static constexpr int kQsOff = kSumOff + 4 * kMaxHeads * 4;               // [HG] f32
-  static constexpr int kStartOff = kQsOff + kMaxHeads * 4;                  // Cursor
-  static constexpr int kScanOff = kStartOff + 32;                           // [8 warps + 1] int64
-  static constexpr int kTmemOff = kScanOff + 80;
+  static constexpr int kStartOff = (kQsOff + kMaxHeads * 4 + 15) / 16 * 16;  // Cursor
+  static constexpr int kSharesOff = (kStartOff + 32 + 15) / 16 * 16;        // Shares
+  static constexpr int kScanOff = kSharesOff + 64;                          // [8 warps] int64
+  static constexpr int kTmemOff = kScanOff + 64;
   static constexpr int kBytes = kTmemOff + 16;
   static constexpr int kAlloc = kBytes + 1024;
   static constexpr int kOCol = 2 * kN;                 // O after the two S buffers
@@ -258,18 +266,34 @@ __device__ __forceinline__ float join_terms(const float* v, int h) {
   return r;
 }
 
+// What the CTAs' shares are made from.
+struct Shares {
+  int64_t weight;  // of all items
+  int64_t ctas;    // that take part
+  int64_t first;   // weight before the item that the CTA's first tile belongs to
+  int64_t tile[2]; // tiles before each end of the CTA's share
+  int item;        // weight of an item beside its tiles
+};
+
 // The CTA's first tile and how many it has, found by all threads: prefix sums
-// of the rows' tiles, then the thread whose rows hold the tile walks them.
+// of the rows' tiles, then the threads whose rows hold the two ends of the
+// CTA's share walk them.
 template <typename L>
 __device__ __forceinline__ Cursor find_start(const Args& a, uint8_t* smem) {
   Cursor* start = reinterpret_cast<Cursor*>(smem + L::kStartOff);
+  Shares* sh = reinterpret_cast<Shares*>(smem + L::kSharesOff);
   int64_t* scan = reinterpret_cast<int64_t*>(smem + L::kScanOff);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t items = (int64_t)a.num_kv_heads * a.head_chunks;
   const int per = (a.num_seqs + kThreads - 1) / kThreads;
   const int s0 = min(a.num_seqs, (int)threadIdx.x * per), s1 = min(a.num_seqs, s0 + per);
+  // tiles, and rows that have any above bit 40
+  constexpr int64_t kRow = (int64_t)1 << 40;
   int64_t sum = 0;
-  for (int s = s0; s < s1; ++s) sum += (context_of(a, s, blockIdx.x == 0) + kTile - 1) / kTile;
+  for (int s = s0; s < s1; ++s) {
+    const int n = (context_of(a, s, blockIdx.x == 0) + kTile - 1) / kTile;
+    sum += n + (n > 0 ? kRow : 0);
+  }
   int64_t incl = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -277,7 +301,6 @@ __device__ __forceinline__ Cursor find_start(const Args& a, uint8_t* smem) {
     if (lane >= o) incl += v;
   }
   if (lane == 31) scan[warp] = incl;
-  if (threadIdx.x == 0) *start = Cursor{0, 0, 0, 0, 0, 0};
   __syncthreads();
   int64_t before = incl - sum, total = 0;
 #pragma unroll
@@ -285,39 +308,48 @@ __device__ __forceinline__ Cursor find_start(const Args& a, uint8_t* smem) {
     if (w < warp) before += scan[w];
     total += scan[w];
   }
+  const int64_t tiles = (total & (kRow - 1)) * items;
   // no more CTAs than tiles take part, so each of them has at least one
-  const int64_t W = total * items, G = W < gridDim.x ? (W > 0 ? W : 1) : gridDim.x;
-  const int64_t b0 = blockIdx.x < G ? W * blockIdx.x / G : W, b1 = blockIdx.x < G ? W * (blockIdx.x + 1) / G : W;
+  const int64_t G = tiles < gridDim.x ? (tiles > 0 ? tiles : 1) : gridDim.x;
+  const int wi = tiles >= kManyTiles * G ? kItemWeight : 0;
+  auto weight = [&](int64_t v) { return items * (kTileWeight * (v & (kRow - 1)) + wi * (v >> 40)); };
+  const int64_t W = weight(total);
   const bool whole = a.meta == nullptr;  // items are not shared: both ends move on to where one begins
-  __syncthreads();  // the scan words have been read: they become the two ends
   if (threadIdx.x == 0) {
-    scan[0] = b0;
-    scan[1] = b1;
-    scan[2] = W;
-    scan[3] = G;
+    *start = Cursor{0, 0, 0, 0, 0, 0};
+    *sh = Shares{W, G, 0, {tiles, tiles}, wi};
   }
   __syncthreads();
-  // tile b lies in the row with items * before <= b < items * (before + its tiles)
-  for (int e = 0; e < (whole ? 2 : 1); ++e) {
-    const int64_t b = e == 0 ? b0 : b1;
-    if (b < items * before || b >= items * (before + sum)) continue;
+#pragma unroll 1
+  for (int e = 0; e < 2; ++e) {
+    const int64_t b = blockIdx.x + e < G ? W * (blockIdx.x + e) / G : W;
+    if (b < weight(before) || b >= weight(before + sum)) continue;
     int64_t at = before;
     for (int s = s0; s < s1; ++s) {
       const int ctx = context_of(a, s, false);
       const int n = (ctx + kTile - 1) / kTile;
-      if (b < items * (at + n)) {
-        const int64_t off = b - items * at;
-        const int64_t up = whole ? (n - off % n) % n : 0;
-        if (e == 0) *start = Cursor{s, (int)((off + up) / n), ctx, n, (int)((off + up) % n), 0};
-        scan[e] = b + up;
+      const int64_t row = n > 0 ? n + kRow : 0;
+      if (b < weight(at + row)) {
+        const uint32_t w = kTileWeight * n + wi;
+        const uint32_t off = (uint32_t)(b - weight(at));  // a row's tiles are far below 2^30
+        uint32_t item = off / w, tile = (off % w + kTileWeight - 1) / kTileWeight;
+        if ((whole && tile > 0) || tile >= (uint32_t)n) {
+          tile = 0;
+          ++item;
+        }
+        sh->tile[e] = items * (at & (kRow - 1)) + (int64_t)item * n + tile;
+        if (e == 0) {
+          *start = Cursor{s, (int)item, ctx, n, (int)tile, 0};
+          sh->first = weight(at) + (int64_t)item * w;
+        }
         break;
       }
-      at += n;
+      at += row;
     }
   }
   __syncthreads();
   Cursor c = *start;
-  c.left = scan[1] - scan[0];
+  c.left = (int)(sh->tile[1] - sh->tile[0]);
   if (c.left > 0 && c.item == items) {  // moved on past the row's last item
     c.item = 0;
     do {
@@ -610,6 +642,8 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
     const uint32_t trow = tmem + ((uint32_t)(32 * warp) << 16);
     bool begun = false;
     uint32_t j = 0;
+    const Shares& sh = *reinterpret_cast<const Shares*>(smem + L::kSharesOff);
+    int64_t at = sh.first;  // weight before the segment's item
     // Warp 0 waits for the others, which sleep at a hardware barrier: polling
     // warps would take the issue slots of the other CTAs' softmax.  A wait
     // that runs out sets *fail; every warp sees it after the next barrier and
@@ -769,12 +803,13 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
         }
       }
       if (!whole && cur.tile == 0 && tok == 0) {
-        // an item begun here and finished by the CTA that has its last tile
-        const int64_t* scan = reinterpret_cast<const int64_t*>(smem + L::kScanOff);
-        const int64_t last = scan[0] + (int64_t)(j - cnt) + cur.tiles - 1;
-        a.meta[blockIdx.x] = make_int4(cur.seq, cur.item, (int)(((last + 1) * scan[3] - 1) / scan[2]), 0);
+        // An item begun here.  CTA c's share begins at c W / G: the last one
+        // to begin at the item's last tile or before has that tile.
+        const int64_t last = at + (int64_t)kTileWeight * (cur.tiles - 1);
+        a.meta[blockIdx.x] = make_int4(cur.seq, cur.item, (int)(((last + 1) * sh.ctas - 1) / sh.weight), 0);
         begun = true;
       }
+      at += (int64_t)kTileWeight * cur.tiles + sh.item;
     }
     if (!ok && lane == 0) block_attn_error(CF_DEVERR_TIMEOUT);
     if (a.meta != nullptr && tok == 0 && !begun) a.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
