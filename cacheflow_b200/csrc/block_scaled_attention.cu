@@ -98,7 +98,8 @@ struct Cursor {
 };
 
 // ---------------------------------------------------------------------------
-// The streaming kernel, 1 to 3 CTAs per SM for the whole launch.
+// The streaming kernel, three CTAs per SM (one at head_dim 256) for the whole
+// launch.
 //
 // Both products run on the stored bytes, tcgen05 kind::f8f6f4 with f32
 // accumulation in tensor memory, the tokens or head dimensions as the 128
@@ -142,15 +143,15 @@ struct Layout {
   static constexpr int kHalf = kBoxes * kBox;         // a tile's K or V
   // K and V have rings of their own: a K stage is free once its QK is done,
   // a V stage an exchange of maxima and a PV later.
-  static constexpr int kMinCtas = D == 128 ? (HG <= 8 ? 3 : 2) : 1;  // per SM
-  static constexpr int kStages = kMinCtas == 3 ? 2 : 3;
+  static constexpr int kMinCtas = D == 128 ? 3 : 1;  // per SM
+  static constexpr int kStages = D == 128 ? 2 : 3;
   // Registers of a softmax thread, and of the others, where the launch's even
-  // share (80 at three CTAs per SM, 128 at two) is too few: what one
-  // warpgroup gives up is at least what the other takes.
-  static constexpr bool kSplitRegs = D == 128 && HG >= 8;
-  static constexpr int kLaunchRegs = kMinCtas == 3 ? 80 : 128;
-  static constexpr int kSoftmaxRegs = kMinCtas == 3 ? 112 : 200;
-  static constexpr int kOtherRegs = kMinCtas == 3 ? 48 : 56;
+  // share of three CTAs per SM is too few: what one warpgroup gives up is at
+  // least what the other takes.
+  static constexpr bool kSplitRegs = D == 128 && HG == 8;
+  static constexpr int kLaunchRegs = 80;
+  static constexpr int kSoftmaxRegs = 112;
+  static constexpr int kOtherRegs = 48;
   static_assert(kSoftmaxRegs + kOtherRegs <= 2 * kLaunchRegs, "more registers than the block has");
   static constexpr int kVOff = kStages * kHalf;
   static constexpr int kQOff = 2 * kStages * kHalf;   // Q: kBoxes x [kN rows x 128 B]
@@ -363,7 +364,7 @@ __device__ __forceinline__ Cursor find_start(const Args& a, uint8_t* smem) {
 
 template <typename T, int D, int HG>
 __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
-    block_attention_kernel(const Args a, const __grid_constant__ CUtensorMap tmk,
+    block_attention_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap tmk,
                            const __grid_constant__ CUtensorMap tmv) {
   using L = Layout<T, D, HG>;
   constexpr int N = L::kN, S = L::kStages, kT = kTerms<T>;
@@ -411,6 +412,10 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
     tmem_relinquish();
   }
   tc_fence_before();
+  // What the launch before this one wrote is read from here on; the join may
+  // be set up beside this kernel.
+  grid_dependency_wait();
+  grid_dependency_launch();
   Cursor cur = find_start<L>(a, smem);  // synchronises the block
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
@@ -814,59 +819,108 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
     if (!ok && lane == 0) block_attn_error(CF_DEVERR_TIMEOUT);
     if (a.meta != nullptr && tok == 0 && !begun) a.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
   }
-  grid_dependency_launch();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   if (warp == kMmaWarp) tmem_dealloc(tmem, L::kTmemCols);
 }
 
-// Joins the items that several CTAs share, one CTA of D threads per (CTA of
-// the streaming kernel, head): the item that CTA c began, its later pieces in
-// the first slots of CTAs c + 1 .. last.
+// Joins the items that several CTAs share, one CTA per CTA c of the streaming
+// kernel: the item that c began, its later pieces in the first slots of CTAs
+// c + 1 .. last.  With few pieces a warp takes a head, with many (a few rows
+// over all CTAs) the warps share each head's; a lane has the maximum and sum
+// of one of 32 pieces, then its columns of all.
 // out = sum_p w_p o_p / sum_p w_p, w_p = sum_p 2^(max_p - max).
+// Latency-bound: three dependent loads (the CTA's entry, the sums, the
+// pieces' outputs) behind a launch that overlaps the streaming kernel's end.
+constexpr int kJoinWarps = 8;
+constexpr int kFewPieces = 8;
+
 template <typename T, int D, int HG>
-__global__ void __launch_bounds__(D) block_attention_join_kernel(const Args a) {
-  extern __shared__ float w_sh[];  // a weight per piece
-  __shared__ float red[2][D / 32];
+__global__ void __launch_bounds__(kJoinWarps * 32) block_attention_join_kernel(const __grid_constant__ Args a) {
+  constexpr int E = D / 32;
+  __shared__ float sm[kJoinWarps], sl[kJoinWarps];
+  __shared__ __align__(16) float so[kJoinWarps][D];
   grid_dependency_wait();
-  const int c = blockIdx.x, h = blockIdx.y;
+  const int c = blockIdx.x;
   const int4 meta = a.meta[c];
   if (meta.x < 0) return;
   const int kvh = meta.y / a.head_chunks, chunk = meta.y - kvh * a.head_chunks;
-  if (h >= min(HG, a.group - chunk * HG)) return;
+  const int nheads = min(HG, a.group - chunk * HG);
   const int pieces = meta.z - c + 1;
-  auto slot = [&](int p) { return (size_t)(p == 0 ? 2 * c + 1 : 2 * (c + p)) * HG + h; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float m = -INFINITY;
-  for (int p = threadIdx.x; p < pieces; p += D) m = fmaxf(m, a.part_max[slot(p)]);
+  T* out = static_cast<T*>(a.out) + ((size_t)meta.x * a.num_heads + kvh * a.group + chunk * HG) * D;
+  float m, l, o[E];
+  auto collect = [&](int h, int first, int stride) {  // pieces first, first + stride, ... of head h
+    auto slot = [&](int p) { return (size_t)(p == 0 ? 2 * c + 1 : 2 * (c + p)) * HG + h; };
+    m = -INFINITY;
+    l = 0.f;
 #pragma unroll
-  for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, shfl_xor(m, i));
-  if (lane == 0) red[0][warp] = m;
-  __syncthreads();
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+    for (int p0 = first; p0 < pieces; p0 += stride * 32) {
+      const int mine = p0 + stride * lane;
+      const float sum = mine < pieces ? a.part_sum[slot(mine)] : 0.f;
+      const float top = mine < pieces ? a.part_max[slot(mine)] : -INFINITY;
+      // a piece without a readable token has sum 0 and maximum -inf
+      const float mn = fmaxf(m, warp_max(top));
+      const float mu = mn == -INFINITY ? 0.f : mn;
+      const float alpha = exp2f(m - mu);
+      m = mn;
+      const float w = sum == 0.f ? 0.f : sum * exp2f(top - mu);
+      float ws = w;
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) m = fmaxf(m, red[0][i]);
-  float l = 0.f;
-  for (int p = threadIdx.x; p < pieces; p += D) {
-    const float sum = a.part_sum[slot(p)];
-    // a piece without a readable token has sum 0 and max -inf
-    const float w = sum == 0.f ? 0.f : sum * exp2f(a.part_max[slot(p)] - m);
-    w_sh[p] = w;
-    l += w;
+      for (int i = 16; i > 0; i >>= 1) ws += shfl_xor(ws, i);
+      l = l * alpha + ws;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] *= alpha;
+      const int n = min(32, (pieces - p0 + stride - 1) / stride);
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const float wp = __shfl_sync(0xffffffffu, w, i);
+        float x[E];
+        load_widen<float, E>(a.part_out + slot(p0 + stride * i) * D + lane * E, x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = fmaf(wp, x[e], o[e]);
+      }
+    }
+  };
+  if (pieces <= kFewPieces) {
+    for (int h = warp; h < nheads; h += kJoinWarps) {
+      collect(h, 0, 1);
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+      for (int e = 0; e < E; ++e) out[h * D + lane * E + e] = from_float<T>(o[e] * inv);
+    }
+    return;
   }
+  for (int h = 0; h < nheads; ++h) {
+    collect(h, warp, kJoinWarps);
+    if (lane == 0) {
+      sm[warp] = m;
+      sl[warp] = l;
+    }
 #pragma unroll
-  for (int i = 16; i > 0; i >>= 1) l += shfl_xor(l, i);
-  if (lane == 0) red[1][warp] = l;
-  __syncthreads();
-  l = 0.f;
+    for (int e = 0; e < E; ++e) so[warp][lane * E + e] = o[e];
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) l += red[1][i];
-  float o = 0.f;
-#pragma unroll 8
-  for (int p = 0; p < pieces; ++p) o = fmaf(w_sh[p], a.part_out[slot(p) * D + threadIdx.x], o);
-  const int head = kvh * a.group + chunk * HG + h;
-  static_cast<T*>(a.out)[((size_t)meta.x * a.num_heads + head) * D + threadIdx.x] =
-      from_float<T>(l == 0.f ? 0.f : o / l);
+    for (int w = 0; w < kJoinWarps; ++w) m = fmaxf(m, sm[w]);
+    const float mu = m == -INFINITY ? 0.f : m;
+    float scale[kJoinWarps];
+    l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) {
+      scale[w] = exp2f(sm[w] - mu);
+      l = fmaf(sl[w], scale[w], l);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    for (int d = threadIdx.x; d < D; d += kJoinWarps * 32) {
+      float r = 0.f;
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) r = fmaf(so[w][d], scale[w], r);
+      out[h * D + d] = from_float<T>(r * inv);
+    }
+    __syncthreads();
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -948,9 +1002,8 @@ cf_status launch_heads(Args a, const BlockScaledLaunch& l) {
   }
   const int64_t want = share ? items * tiles : items;
   const unsigned grid = (unsigned)(want < ctas ? want : ctas);
-  block_attention_kernel<T, D, HG><<<grid, kThreads, Layout<T, D, HG>::kAlloc, l.stream>>>(a, mk, mv);
-  st = check_launch();
-  if (st != CF_OK || !share) return st;
+  // Both launches may begin under the end of what is before them in the
+  // stream; each waits for it before it touches memory.
   cudaLaunchConfig_t cfg = {};
   cfg.stream = l.stream;
   cudaLaunchAttribute attr[1];
@@ -958,14 +1011,20 @@ cf_status launch_heads(Args a, const BlockScaledLaunch& l) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cfg.gridDim = dim3(grid, (unsigned)(a.group < HG ? a.group : HG));
-  cfg.blockDim = dim3(D);
-  cfg.dynamicSmemBytes = grid * sizeof(float);
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Layout<T, D, HG>::kAlloc;
+  st = cuda_status(cudaLaunchKernelEx(&cfg, block_attention_kernel<T, D, HG>, a, mk, mv));
+  if (st != CF_OK || !share) return st;
+  cfg.dynamicSmemBytes = 0;
+  cfg.blockDim = dim3(kJoinWarps * 32);
   return cuda_status(cudaLaunchKernelEx(&cfg, block_attention_join_kernel<T, D, HG>, a));
 }
 
 // Calls f with the kernel's types as template arguments: HG query heads of a
-// KV head per item.
+// KV head per item, larger groups in chunks of 8 (16 heads in one item left
+// room for two CTAs per SM: 64 rows of 1024-8192 tokens 89 us, 83 as two
+// items, whose KV bytes meet in L2).
 template <typename F>
 auto dispatch(const cf_paged_attention_params& p, F&& f) {
   const int group = p.num_heads / p.num_kv_heads;
@@ -974,8 +1033,7 @@ auto dispatch(const cf_paged_attention_params& p, F&& f) {
     constexpr int D = decltype(d)::value;
     if (group == 1) return f.template operator()<Tp, D, 1>();
     if (group <= 4) return f.template operator()<Tp, D, 4>();
-    if (group <= 8) return f.template operator()<Tp, D, 8>();
-    return f.template operator()<Tp, D, 16>();
+    return f.template operator()<Tp, D, 8>();
   };
   using D128 = std::integral_constant<int, 128>;
   using D256 = std::integral_constant<int, 256>;
