@@ -181,8 +181,8 @@ SIGNATURES = {
     ),
     "cf_reshape_and_cache_fp8_block": (
         c_int32,
-        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32,
-         c_int64, c_int32, c_void_p],
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int64,
+         c_int64, c_int32, c_int64, c_int32, c_void_p],
     ),
     "cf_paged_attention_fp8_block_v1": (
         c_int32, [POINTER(AttentionParams), c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],

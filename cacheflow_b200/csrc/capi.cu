@@ -507,6 +507,7 @@ cf_status cf_reshape_and_cache_fp8_block(const void* key, const void* value, voi
                                          void* value_cache, float* k_scales, float* v_scales,
                                          const int32_t* slot_mapping, int32_t num_tokens,
                                          int32_t num_kv_heads, int32_t head_dim,
+                                         int64_t key_stride, int64_t value_stride,
                                          int32_t block_size, int64_t num_blocks, int32_t dtype,
                                          void* stream) {
   if ((dtype != CF_F32 && dtype != CF_F16 && dtype != CF_BF16) || num_tokens < 0 ||
@@ -524,7 +525,8 @@ cf_status cf_reshape_and_cache_fp8_block(const void* key, const void* value, voi
   cf_rope_params p = {};
   p.key = key;
   p.value = value;
-  p.key_stride[0] = p.value_stride[0] = (int64_t)num_kv_heads * head_dim;
+  p.key_stride[0] = key_stride;
+  p.value_stride[0] = value_stride;
   p.key_stride[1] = p.value_stride[1] = head_dim;
   p.num_tokens = num_tokens;
   p.num_kv_heads = num_kv_heads;

@@ -17,6 +17,8 @@
 //
 // Bound: HBM.  A row is read once and written once; the table row of a token
 // (R floats) is shared by all its heads.
+#include <initializer_list>
+
 #include "cf_device.cuh"
 #include "cf_internal.h"
 
@@ -158,11 +160,13 @@ struct Unit {
   bool rot, has1, has2;
 };
 
-template <int V, bool IL>
+// kFull: every lane of a row has a unit that rotates (R = D, a power of two
+// of units), known at compile time.
+template <int V, bool IL, bool kFull>
 __device__ __forceinline__ Unit unit_of(const RopeArgs& a, int u) {
   Unit x;
-  x.rot = u < a.rot_units;
-  x.has1 = u < a.units;
+  x.rot = kFull || u < a.rot_units;
+  x.has1 = kFull || u < a.units;
   if (x.rot) {
     x.o1 = IL ? 2 * u * V : u * V;
     x.o2 = IL ? x.o1 + V : a.rotary / 2 + x.o1;
@@ -175,14 +179,44 @@ __device__ __forceinline__ Unit unit_of(const RopeArgs& a, int u) {
   return x;
 }
 
-template <int V, bool IL>
-__device__ __forceinline__ void rotate(float* f, const float* cs, const float* sn) {  // f[0..V) and f[V..2V)
+// What a lane multiplies its pairs (a, b) with, weights and angles in one:
+//   a' = a ca - b sb,  b' = b cb + a sa   (columns that do not rotate: a ca, b cb)
+template <int V>
+struct Turn {
+  float ca[V], cb[V], sa[V], sb[V];
+};
+
+template <typename T, int V, int K, bool IL>
+__device__ __forceinline__ void load_turn(const RopeArgs& a, const void* w, int pos, int lane, const Unit (&un)[K],
+                                          Turn<V> (&tn)[K]) {
+  const float* row = a.positions != nullptr ? a.cos_sin + (size_t)pos * a.rotary : nullptr;
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int ia = IL ? 2 * i : i, ib = IL ? 2 * i + 1 : V + i;
-    const float x = f[ia], y = f[ib];
-    f[ia] = fmaf(x, cs[i], -(y * sn[i]));
-    f[ib] = fmaf(y, cs[i], x * sn[i]);
+  for (int k = 0; k < K; ++k) {
+    float c[V], s[V], g[2 * V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      c[i] = 1.f;
+      s[i] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * V; ++i) g[i] = 1.f;
+    if (un[k].rot && row != nullptr) {
+      const int i = (lane + (k << a.lanes_log2)) * V;
+      load_f32<V>(row + i, c);
+      load_f32<V>(row + a.rotary / 2 + i, s);
+    }
+    if (w != nullptr) {
+      if (un[k].has1) load_weight<T, V>(a, w, un[k].o1, g);
+      if (un[k].has2) load_weight<T, V>(a, w, un[k].o2, g + V);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float ga = IL ? g[2 * i] : g[i], gb = IL ? g[2 * i + 1] : g[V + i];
+      tn[k].ca[i] = ga * c[i];
+      tn[k].cb[i] = gb * c[i];
+      tn[k].sa[i] = ga * s[i];
+      tn[k].sb[i] = gb * s[i];
+    }
   }
 }
 
@@ -192,171 +226,167 @@ __device__ __forceinline__ float row_sum(float v, int log2) {
   return v;
 }
 
-// The lane's K units of one row, normed (w not null) and rotated (rot), in
-// f32.  Every lane of the warp calls it: the rows of a warp may differ in
-// having a weight, and the sum runs across lanes.
-template <typename T, int V, int K, bool IL>
-__device__ __forceinline__ void norm_rotate(const RopeArgs& a, float (&f)[K][2 * V], const void* w, bool rot,
-                                            const Unit (&un)[K], const float (&cs)[K][V], const float (&sn)[K][V]) {
-  if (a.q_w != nullptr || a.k_w != nullptr) {
-    float ss = 0.f;
+// The lane's K units of one Q or K row, normed (if the row kind has a weight:
+// the same for the whole warp) and turned, in f32.
+template <int V, int K, bool IL>
+__device__ __forceinline__ void norm_turn(const RopeArgs& a, float (&f)[K][2 * V], bool norm, const Unit (&un)[K],
+                                          const Turn<V> (&tn)[K]) {
+  float rs = 1.f;
+  if (norm) {
+    float s0 = 0.f, s1 = 0.f;  // two chains
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < 2 * V; ++i) ss = fmaf(f[k][i], f[k][i], ss);
-    ss = row_sum(ss, a.lanes_log2);
-    if (w != nullptr) {
-      const float rs = rsqrtf(ss / (float)a.head_dim + a.eps);
+      for (int i = 0; i < V; ++i) {
+        s0 = fmaf(f[k][i], f[k][i], s0);
+        s1 = fmaf(f[k][V + i], f[k][V + i], s1);
+      }
+    rs = rsqrtf(row_sum(s0 + s1, a.lanes_log2) / (float)a.head_dim + a.eps);
+  }
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        float g[V];
-        if (un[k].has1) {
-          load_weight<T, V>(a, w, un[k].o1, g);
+  for (int k = 0; k < K; ++k) {
+    const Turn<V>& t = tn[k];
 #pragma unroll
-          for (int i = 0; i < V; ++i) f[k][i] = f[k][i] * rs * g[i];
-        }
-        if (un[k].has2) {
-          load_weight<T, V>(a, w, un[k].o2, g);
-#pragma unroll
-          for (int i = 0; i < V; ++i) f[k][V + i] = f[k][V + i] * rs * g[i];
-        }
+    for (int i = 0; i < V; ++i) {
+      const int ia = IL ? 2 * i : i, ib = IL ? 2 * i + 1 : V + i;
+      float& x = f[k][ia];
+      float& y = f[k][ib];
+      const float xa = x, yb = y;
+      if (un[k].rot) {
+        x = fmaf(xa, t.ca[i], -(yb * t.sb[i]));
+        y = fmaf(yb, t.cb[i], xa * t.sa[i]);
+      } else {
+        x = xa * t.ca[i];
+        y = yb * t.cb[i];
+      }
+      if (norm) {
+        x *= rs;
+        y *= rs;
       }
     }
   }
-  if (rot) {
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-      if (un[k].rot) rotate<V, IL>(f[k], cs[k], sn[k]);
-  }
-}
-
-template <int V, int K>
-__device__ __forceinline__ void load_angles(const RopeArgs& a, int pos, int lane, const Unit (&un)[K],
-                                            float (&cs)[K][V], float (&sn)[K][V]) {
-  const float* row = a.cos_sin + (size_t)pos * a.rotary;
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    if (un[k].rot) {
-      const int i = (lane + (k << a.lanes_log2)) * V;
-      load_f32<V>(row + i, cs[k]);
-      load_f32<V>(row + a.rotary / 2 + i, sn[k]);
-    }
-  }
 }
 
 // ---------------------------------------------------------------------------
-// Row items.  A warp takes 32 / lanes rows of one token at a time, U times
-// over: the token's angles are loaded once for all of them, and their 2U
-// loads per lane are in flight together.  Rows: the query heads, then the K
-// heads, then (cache destinations) the V heads; `nrows` of them.
+// Row items.  A warp takes 32 / lanes heads of one token and one kind (Q, K
+// or V) at a time, U times over: the token's angles and the kind's weights are
+// loaded and multiplied once for all of them, every branch on the kind is the
+// whole warp's, and the 2U loads per lane are in flight together.
 // ---------------------------------------------------------------------------
-template <typename T, int V, int K, int U, bool IL>
-__device__ __forceinline__ void row_items(const RopeArgs& a, int64_t warp, int64_t num_warps, int nrows) {
+template <typename T, int V, int K, int U, bool IL, bool kFull>
+__device__ __forceinline__ void row_items(const RopeArgs& a, int64_t warp, int64_t num_warps, bool with_kv) {
   const int lane = threadIdx.x & 31;
   const int sub = lane & ((1 << a.lanes_log2) - 1);
   const int per_warp = 32 >> a.lanes_log2;
   const int grp = lane >> a.lanes_log2;
-  const int per_token = (nrows + per_warp * U - 1) / (per_warp * U);
-  const int64_t items = (int64_t)a.num_tokens * per_token;
+  const int nq = (a.num_heads + per_warp * U - 1) / (per_warp * U);
+  const int nk = with_kv ? (a.num_kv_heads + per_warp * U - 1) / (per_warp * U) : 0;
+  const int per_token = nq + nk + (a.dest == kDense ? 0 : nk);
   Unit un[K];
 #pragma unroll
-  for (int k = 0; k < K; ++k) un[k] = unit_of<V, IL>(a, sub + (k << a.lanes_log2));
+  for (int k = 0; k < K; ++k) un[k] = unit_of<V, IL, kFull>(a, sub + (k << a.lanes_log2));
 
-  for (int64_t item = warp; item < items; item += num_warps) {
-    const int64_t t = item / per_token;
-    const int row0 = (int)(item - t * per_token) * per_warp * U + grp;
+  // item = t * per_token + c, advanced without a division
+  int64_t t = warp / per_token;
+  int c = (int)(warp - t * per_token);
+  const int64_t dt = num_warps / per_token;
+  const int dc = (int)(num_warps - dt * per_token);
+  for (; t < a.num_tokens; t += dt, c += dc) {
+    if (c >= per_token) {
+      c -= per_token;
+      if (++t >= a.num_tokens) break;
+    }
+    const int kind = c < nq ? 0 : (c < nq + nk ? 1 : 2);
+    const int heads = kind == 0 ? a.num_heads : a.num_kv_heads;
+    const int head0 = (kind == 0 ? c : kind == 1 ? c - nq : c - nq - nk) * per_warp * U + grp;
+    const void* base = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+    const int64_t ts = kind == 0 ? a.q_ts : kind == 1 ? a.k_ts : a.v_ts;
+    const int64_t hs = kind == 0 ? a.q_hs : kind == 1 ? a.k_hs : a.v_hs;
     int pos = 0;
     if (a.positions != nullptr) pos = a.positions[t];
     int64_t slot = -1;
-    if (a.slots != nullptr) slot = a.slots[t];
+    if (a.slots != nullptr && kind > 0) slot = a.slots[t];
+    const T* src = static_cast<const T*>(base) + t * ts + head0 * hs;
     Raw<T, V> raw[U][K][2];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int r = row0 + u * per_warp;
-      if (r >= nrows) continue;
-      const T* src;
-      if (r < a.num_heads)
-        src = static_cast<const T*>(a.q) + t * a.q_ts + r * a.q_hs;
-      else if (r < a.num_heads + a.num_kv_heads)
-        src = static_cast<const T*>(a.k) + t * a.k_ts + (r - a.num_heads) * a.k_hs;
-      else
-        src = static_cast<const T*>(a.v) + t * a.v_ts + (r - a.num_heads - a.num_kv_heads) * a.v_hs;
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        if (un[k].has1) raw[u][k][0] = *reinterpret_cast<const Raw<T, V>*>(src + un[k].o1);
-        if (un[k].has2) raw[u][k][1] = *reinterpret_cast<const Raw<T, V>*>(src + un[k].o2);
-      }
-    }
-    const bool first = row0 - grp == 0 && lane == 0;
-    if (a.positions != nullptr) {
-      if (pos >= a.max_positions && first) rope_error(CF_DEVERR_POSITION);
-      if (pos < 0 || pos >= a.max_positions) continue;  // a padding token, or one without angles: left out whole
-    }
-    if (slot >= a.num_slots) {
-      if (first) rope_error(CF_DEVERR_SLOT);
-      slot = -1;
-    }
-    float cs[K][V], sn[K][V];
-    if (a.positions != nullptr) load_angles<V, K>(a, pos, sub, un, cs, sn);
-    const int64_t blk = slot >= 0 ? slot / a.block_size : 0;
-    const int64_t off = slot - blk * a.block_size;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int r = row0 + u * per_warp;
-      const bool valid = r < nrows;
-      const int kind = r < a.num_heads ? 0 : (r < a.num_heads + a.num_kv_heads ? 1 : 2);
-      const int head = kind == 0 ? r : (kind == 1 ? r - a.num_heads : r - a.num_heads - a.num_kv_heads);
-      float f[K][2 * V];
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-#pragma unroll
-        for (int i = 0; i < 2 * V; ++i) f[k][i] = 0.f;
-        if (valid && un[k].has1) unpack<T, V>(raw[u][k][0], f[k]);
-        if (valid && un[k].has2) unpack<T, V>(raw[u][k][1], f[k] + V);
-      }
-      norm_rotate<T, V, K, IL>(a, f, kind == 0 ? a.q_w : (kind == 1 ? a.k_w : nullptr), kind < 2, un, cs, sn);
-      if (!valid) continue;
-      if (kind > 0 && a.dest != kDense) {
-        if (slot < 0) continue;  // a padding row: nothing is appended
-        const int64_t row = ((blk * a.num_kv_heads + head) * a.block_size + off) * a.head_dim;
-        if (a.dest == kCacheFp8) {
-          uint8_t* dst = static_cast<uint8_t*>(kind == 1 ? a.kc : a.vc) + row;
-          const float sc = kind == 1 ? a.k_scale : a.v_scale;
-#pragma unroll
-          for (int k = 0; k < K; ++k) {
-#pragma unroll
-            for (int i = 0; i < 2 * V; ++i) f[k][i] = __fdiv_rn(f[k][i], sc);
-            if (un[k].has1) store_e4m3<V>(dst + un[k].o1, f[k]);
-            if (un[k].has2) store_e4m3<V>(dst + un[k].o2, f[k] + V);
-          }
-        } else {
-          T* dst = static_cast<T*>(kind == 1 ? a.kc : a.vc) + row;
-#pragma unroll
-          for (int k = 0; k < K; ++k) {
-            // V is moved as it is, bit for bit
-            if (un[k].has1)
-              *reinterpret_cast<Raw<T, V>*>(dst + un[k].o1) = kind == 2 ? raw[u][k][0] : pack<T, V>(f[k]);
-            if (un[k].has2)
-              *reinterpret_cast<Raw<T, V>*>(dst + un[k].o2) = kind == 2 ? raw[u][k][1] : pack<T, V>(f[k] + V);
-          }
-        }
-      } else {
-        T* dst = kind == 0 ? static_cast<T*>(a.q_out) + t * a.qo_ts + head * a.qo_hs
-                           : static_cast<T*>(a.k_out) + t * a.ko_ts + head * a.ko_hs;
+      if (head0 + u * per_warp < heads) {
+        const T* p = src + (int64_t)(u * per_warp) * hs;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-          if (un[k].has1) *reinterpret_cast<Raw<T, V>*>(dst + un[k].o1) = pack<T, V>(f[k]);
-          if (un[k].has2) *reinterpret_cast<Raw<T, V>*>(dst + un[k].o2) = pack<T, V>(f[k] + V);
+          if (un[k].has1) raw[u][k][0] = *reinterpret_cast<const Raw<T, V>*>(p + un[k].o1);
+          if (un[k].has2) raw[u][k][1] = *reinterpret_cast<const Raw<T, V>*>(p + un[k].o2);
+        }
+      }
+    }
+    if (a.positions != nullptr) {
+      if (pos >= a.max_positions && lane == 0) rope_error(CF_DEVERR_POSITION);
+      if (pos < 0 || pos >= a.max_positions) continue;  // a padding token, or one without angles: left out whole
+    }
+    const bool cached = kind > 0 && a.dest != kDense;
+    if (cached) {
+      if (slot >= a.num_slots && lane == 0) rope_error(CF_DEVERR_SLOT);
+      if (slot < 0 || slot >= a.num_slots) continue;  // a padding row: nothing is appended
+    }
+    const void* w = kind == 0 ? a.q_w : kind == 1 ? a.k_w : nullptr;
+    Turn<V> tn[K];
+    if (kind < 2) load_turn<T, V, K, IL>(a, w, pos, sub, un, tn);
+    // the rows' destination, element strides as the source's
+    const int64_t blk = cached ? slot / a.block_size : 0;
+    const int64_t dhs = cached ? (int64_t)a.block_size * a.head_dim : kind == 0 ? a.qo_hs : a.ko_hs;
+    const int64_t d0 = cached ? (blk * a.num_kv_heads * a.block_size + (slot - blk * a.block_size)) * a.head_dim
+                              : kind == 0 ? t * a.qo_ts : t * a.ko_ts;
+    void* dbase = cached ? (kind == 1 ? a.kc : a.vc) : kind == 0 ? a.q_out : a.k_out;
+    const bool fp8 = cached && a.dest == kCacheFp8;
+    const float sc = kind == 1 ? a.k_scale : a.v_scale;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int head = head0 + u * per_warp;
+      if (u > 0 && head - grp >= heads) break;  // for the whole warp
+      const bool valid = head < heads;
+      float f[K][2 * V];
+      if (kind < 2 || fp8) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          if (!kFull || !valid) {
+#pragma unroll
+            for (int i = 0; i < 2 * V; ++i) f[k][i] = 0.f;
+          }
+          if (valid && un[k].has1) unpack<T, V>(raw[u][k][0], f[k]);
+          if (valid && un[k].has2) unpack<T, V>(raw[u][k][1], f[k] + V);
+        }
+        if (kind < 2) norm_turn<V, K, IL>(a, f, w != nullptr, un, tn);
+      }
+      if (!valid) continue;
+      const int64_t row = d0 + head * dhs;
+      if (fp8) {
+        uint8_t* dst = static_cast<uint8_t*>(dbase) + row;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+#pragma unroll
+          for (int i = 0; i < 2 * V; ++i) f[k][i] = __fdiv_rn(f[k][i], sc);
+          if (un[k].has1) store_e4m3<V>(dst + un[k].o1, f[k]);
+          if (un[k].has2) store_e4m3<V>(dst + un[k].o2, f[k] + V);
+        }
+      } else {
+        T* dst = static_cast<T*>(dbase) + row;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          // V is moved as it is, bit for bit
+          if (un[k].has1)
+            *reinterpret_cast<Raw<T, V>*>(dst + un[k].o1) = kind == 2 ? raw[u][k][0] : pack<T, V>(f[k]);
+          if (un[k].has2)
+            *reinterpret_cast<Raw<T, V>*>(dst + un[k].o2) = kind == 2 ? raw[u][k][1] : pack<T, V>(f[k] + V);
         }
       }
     }
   }
 }
 
-template <typename T, int V, int K, int U, bool IL>
-__global__ void __launch_bounds__(kThreads) rope_rows_kernel(const RopeArgs a) {
-  row_items<T, V, K, U, IL>(a, (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5), (int64_t)gridDim.x * kWarps,
-                            a.num_heads + a.num_kv_heads * (a.dest == kDense ? 1 : 2));
+template <typename T, int V, int K, int U, bool IL, bool kFull>
+__global__ void __launch_bounds__(kThreads) rope_rows_kernel(const __grid_constant__ RopeArgs a) {
+  row_items<T, V, K, U, IL, kFull>(a, (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5), (int64_t)gridDim.x * kWarps,
+                                   true);
 }
 
 // ---------------------------------------------------------------------------
@@ -385,6 +415,7 @@ __global__ void __launch_bounds__(kThreads) rope_rows_kernel(const RopeArgs a) {
 // ---------------------------------------------------------------------------
 constexpr int kBlk = 16;  // tokens of a KV block
 constexpr int kPiece = 16384;
+constexpr int kHeads = 16;  // heads a CTA works on between two block barriers
 
 struct BlockArgs {
   RopeArgs r;
@@ -403,8 +434,10 @@ struct BlockSmem {
   int32_t row_tok[kBlk * kBlk]; // the rows to append: token, and l * 16 + off
   int32_t row_lo[kBlk * kBlk];
   int32_t count[kWarps];
-  uint32_t top[3][2][kBlk];     // max |x| of each block's rows, as f32 bits (K, V)
-  float old[3][2][kBlk];
+  int32_t state[kBlk];          // of a block: its rows in the call, as bits; 0 where it is not this CTA's
+  uint32_t top[2][kHeads][kBlk]; // (K, V), heads at a time: max |x| of a block's rows, as f32 bits
+  float old[2][kHeads][kBlk];    // its scale before the call
+  float now[2][kHeads][kBlk];    // and after it
 };
 
 // The smallest power of two s >= 2^-126 with x <= 448 s; 0 for 0.
@@ -417,19 +450,12 @@ __device__ __forceinline__ float block_scale(uint32_t bits) {
   return __uint_as_float((uint32_t)e << 23);
 }
 
-__device__ __forceinline__ float div_scale(float x, float s) {
-  // x * 2^-k is exact; a pool may also hold scales that are no powers of two
-  const uint32_t b = __float_as_uint(s);
-  if ((b & 0x7fffffu) == 0u && b >= (1u << 23) && b < (254u << 23)) return x * __uint_as_float((254u << 23) - b);
-  return __fdiv_rn(x, s);
-}
-
-template <typename T, int V, int K, bool IL>
-__global__ void __launch_bounds__(kThreads) rope_block_append_kernel(const BlockArgs b) {
+template <typename T, int V, int K, bool IL, bool kFull>
+__global__ void __launch_bounds__(kThreads) rope_block_append_kernel(const __grid_constant__ BlockArgs b) {
   const RopeArgs& a = b.r;
   if ((int)blockIdx.x >= b.kv_ctas) {
-    row_items<T, V, K, K == 1 ? 4 : 1, IL>(a, (int64_t)(blockIdx.x - b.kv_ctas) * kWarps + (threadIdx.x >> 5),
-                                           (int64_t)(gridDim.x - b.kv_ctas) * kWarps, a.num_heads);
+    row_items<T, V, K, K == 1 ? 4 : 1, IL, kFull>(a, (int64_t)(blockIdx.x - b.kv_ctas) * kWarps + (threadIdx.x >> 5),
+                                                  (int64_t)(gridDim.x - b.kv_ctas) * kWarps, false);
     return;
   }
   __shared__ BlockSmem sm;
@@ -466,18 +492,27 @@ __global__ void __launch_bounds__(kThreads) rope_block_append_kernel(const Block
   }
   if (__syncthreads_or(leads ? 1 : 0) == 0) return;  // padding only
 
-  // 2. their tokens, wherever they are in the call
-  for (int i = tid; i < T_; i += kThreads) {
-    const int slot = a.slots[i];
-    if (slot < 0) continue;
-    const int k = slot / kBlk;
-    if (!((sm.filter[(k >> 5) & 31] >> (k & 31)) & 1u)) continue;
-    for (int l = 0; l < kBlk; ++l) {
-      if (sm.lead[l] != k) continue;
-      if (i < w0)
-        sm.dead[l] = 1;
-      else
-        atomicMax(&sm.win[l][slot % kBlk], i);
+  // 2. their tokens, wherever they are in the call (16 loads in flight)
+  constexpr int kLook = 16;
+  for (int i0 = tid; i0 < T_; i0 += kThreads * kLook) {
+    int slot[kLook];
+#pragma unroll
+    for (int u = 0; u < kLook; ++u) {
+      const int i = i0 + u * kThreads;
+      slot[u] = i < T_ ? a.slots[i] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kLook; ++u) {
+      if (slot[u] < 0) continue;
+      const int k = slot[u] / kBlk, i = i0 + u * kThreads;
+      if (!((sm.filter[(k >> 5) & 31] >> (k & 31)) & 1u)) continue;
+      for (int l = 0; l < kBlk; ++l) {
+        if (sm.lead[l] != k) continue;
+        if (i < w0)
+          sm.dead[l] = 1;
+        else
+          atomicMax(&sm.win[l][slot[u] % kBlk], i);
+      }
     }
   }
   __syncthreads();
@@ -508,125 +543,162 @@ __global__ void __launch_bounds__(kThreads) rope_block_append_kernel(const Block
       sm.row_tok[at] = tok;
       sm.row_lo[at] = tid;
     }
+    if ((lane & 15) == 0) sm.state[l] = (int32_t)((there >> lane) & 0xffffu);
   }
   __syncthreads();
 
-  // 4. head by head: warps 0-3 take the K rows, warps 4-7 the V rows
-  const int kv = warp >= kWarps / 2 ? 1 : 0;
-  const int ht = tid & (kThreads / 2 - 1);
+  // 4. the rows, kHeads heads at a time: maxima, scales, bytes.  A warp takes
+  // 32 / lanes rows of K or V and walks the heads, so the rows' angles and the
+  // weights are loaded once; where that leaves warps over, they share the
+  // heads.  The second walk loads and turns the rows again (they are in L1)
+  // unless there was one head to each warp.
   const int sub = lane & ((1 << a.lanes_log2) - 1);
-  const int row_in_pass = ht >> a.lanes_log2;
-  const int per_pass = (kThreads / 2) >> a.lanes_log2;
-  const int passes = (n + per_pass - 1) / per_pass;
+  const int per_warp = 32 >> a.lanes_log2;
+  const int groups = (n + per_warp - 1) / per_warp;
+  const int sharing = max(1, kWarps / (2 * groups));  // warps per (K or V, group of rows)
   Unit un[K];
 #pragma unroll
-  for (int k = 0; k < K; ++k) un[k] = unit_of<V, IL>(a, sub + (k << a.lanes_log2));
-  float* scales = kv ? b.v_scales : b.k_scales;
-  uint8_t* cache = static_cast<uint8_t*>(kv ? a.vc : a.kc);
-  const T* src = static_cast<const T*>(kv ? a.v : a.k);
-  const int64_t ts = kv ? a.v_ts : a.k_ts, hs = kv ? a.v_hs : a.k_hs;
+  for (int k = 0; k < K; ++k) un[k] = unit_of<V, IL, kFull>(a, sub + (k << a.lanes_log2));
 
-  float cs[K][V], sn[K][V], f[K][2 * V];
-  auto load = [&](int e, int head) {  // row e of the list, normed and rotated
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < 2 * V; ++i) f[k][i] = 0.f;
+  Raw<T, V> raw[K][2];
+  Turn<V> tn[K];
+  float f[K][2 * V];
+  auto fetch = [&](int kv, int e, int head) {  // row e of the list
     if (e < n) {
-      const T* p = src + (int64_t)sm.row_tok[e] * ts + (int64_t)head * hs;
+      const T* p = static_cast<const T*>(kv ? a.v : a.k) + (int64_t)sm.row_tok[e] * (kv ? a.v_ts : a.k_ts) +
+                   (int64_t)head * (kv ? a.v_hs : a.k_hs);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        if (un[k].has1) unpack<T, V>(*reinterpret_cast<const Raw<T, V>*>(p + un[k].o1), f[k]);
-        if (un[k].has2) unpack<T, V>(*reinterpret_cast<const Raw<T, V>*>(p + un[k].o2), f[k] + V);
+        if (un[k].has1) raw[k][0] = *reinterpret_cast<const Raw<T, V>*>(p + un[k].o1);
+        if (un[k].has2) raw[k][1] = *reinterpret_cast<const Raw<T, V>*>(p + un[k].o2);
       }
     }
-    if (kv == 0) norm_rotate<T, V, K, IL>(a, f, a.k_w, e < n && a.positions != nullptr, un, cs, sn);
   };
-  auto angles = [&](int e) {
-    if (kv == 0 && e < n && a.positions != nullptr)
-      load_angles<V, K>(a, a.positions[sm.row_tok[e]], sub, un, cs, sn);
+  auto turns = [&](int kv) { return kv == 0 && (a.k_w != nullptr || a.positions != nullptr); };
+  auto angles = [&](int kv, int e) {
+    if (turns(kv) && e < n)
+      load_turn<T, V, K, IL>(a, a.k_w, a.positions != nullptr ? a.positions[sm.row_tok[e]] : 0, sub, un, tn);
   };
-  angles(row_in_pass);
-  int buf = 0;
-  for (int head = blockIdx.x % b.head_split; head < a.num_kv_heads; head += b.head_split) {
-    const int next = buf == 2 ? 0 : buf + 1;
-    if (ht < kBlk) {
-      const int blk = sm.dead[ht] ? -1 : sm.lead[ht];
-      float s = blk >= 0 ? scales[(int64_t)blk * a.num_kv_heads + head] : 0.f;
-      sm.old[buf][kv][ht] = s > 0.f && s < INFINITY ? s : 0.f;
-      sm.top[next][kv][ht] = 0u;
+  auto values = [&](int kv, int e) {  // what was fetched, normed and turned
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+#pragma unroll
+      for (int i = 0; i < 2 * V; ++i) f[k][i] = 0.f;
+      if (e < n && un[k].has1) unpack<T, V>(raw[k][0], f[k]);
+      if (e < n && un[k].has2) unpack<T, V>(raw[k][1], f[k] + V);
     }
-    for (int p = 0; p < passes; ++p) {
-      const int e = p * per_pass + row_in_pass;
-      if (passes > 1) angles(e);
-      load(e, head);
-      float top = 0.f;
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < 2 * V; ++i) {
-          const float x = fabsf(f[k][i]);
-          top = fmaxf(top, x <= 3.402823466e38f ? x : 0.f);
-        }
-      for (int m = (1 << a.lanes_log2) >> 1; m > 0; m >>= 1) top = fmaxf(top, shfl_xor(top, m));
-      if (e < n && sub == 0) atomicMax(&sm.top[buf][kv][sm.row_lo[e] / kBlk], __float_as_uint(top));
+    if (turns(kv)) norm_turn<V, K, IL>(a, f, a.k_w != nullptr, un, tn);
+  };
+  const int mine = blockIdx.x % b.head_split;  // heads mine, mine + head_split, ...
+  const int heads = (a.num_kv_heads - mine + b.head_split - 1) / b.head_split;
+  for (int h0 = 0; h0 < heads; h0 += kHeads) {
+    const int nh = min(kHeads, heads - h0);
+    auto head_of = [&](int i) { return mine + (h0 + i) * b.head_split; };
+    if (h0 > 0) __syncthreads();
+    for (int i = tid; i < 2 * kHeads * kBlk; i += kThreads) {
+      const int kv = i / (kHeads * kBlk), hi = i / kBlk % kHeads, l = i % kBlk;
+      float s = 0.f;
+      if (hi < nh && sm.state[l] != 0)
+        s = (kv ? b.v_scales : b.k_scales)[(int64_t)sm.lead[l] * a.num_kv_heads + head_of(hi)];
+      sm.old[kv][hi][l] = s > 0.f && s < INFINITY ? s : 0.f;
+      sm.top[kv][hi][l] = 0u;
     }
     __syncthreads();
-    for (int p = 0; p < passes; ++p) {
-      const int e = p * per_pass + row_in_pass;
-      if (passes > 1) {
-        angles(e);
-        load(e, head);
+    const bool once = 2 * groups * sharing <= kWarps && nh <= sharing;
+    auto walk = [&](auto&& work) {
+      for (int c = warp; c < 2 * groups * sharing; c += kWarps) {
+        const int kv = c % 2, e = c / 2 % groups * per_warp + (lane >> a.lanes_log2);
+        work(kv, e, c / (2 * groups));
       }
-      if (e >= n) continue;
-      const int l = sm.row_lo[e] / kBlk, off = sm.row_lo[e] % kBlk;
-      const float need = block_scale(sm.top[buf][kv][l]);
-      const float s = sm.win[l][0] >= 0 ? need : fmaxf(sm.old[buf][kv][l], need);
-      uint8_t* dst = cache + (((int64_t)sm.lead[l] * a.num_kv_heads + head) * kBlk + off) * a.head_dim;
-      if (s > 0.f) {
+    };
+    walk([&](int kv, int e, int share) {
+      angles(kv, e);
+      if (share < nh) fetch(kv, e, head_of(share));
+      for (int hi = share; hi < nh; hi += sharing) {
+        values(kv, e);
+        if (hi + sharing < nh) fetch(kv, e, head_of(hi + sharing));
+        float top = 0.f;
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-          for (int i = 0; i < 2 * V; ++i) f[k][i] = div_scale(f[k][i], s);
+          for (int i = 0; i < 2 * V; ++i) {
+            const float x = fabsf(f[k][i]);
+            top = fmaxf(top, x <= 3.402823466e38f ? x : 0.f);
+          }
+        for (int m = (1 << a.lanes_log2) >> 1; m > 0; m >>= 1) top = fmaxf(top, shfl_xor(top, m));
+        if (e < n && sub == 0) atomicMax(&sm.top[kv][hi][sm.row_lo[e] / kBlk], __float_as_uint(top));
       }
+    });
+    __syncthreads();
+    for (int i = tid; i < 2 * kHeads * kBlk; i += kThreads) {
+      const int kv = i / (kHeads * kBlk), hi = i / kBlk % kHeads, l = i % kBlk;
+      if (hi >= nh || sm.state[l] == 0) continue;
+      const float need = block_scale(sm.top[kv][hi][l]);
+      const float s = (sm.state[l] & 1) != 0 ? need : fmaxf(sm.old[kv][hi][l], need);
+      sm.now[kv][hi][l] = s;
+      (kv ? b.v_scales : b.k_scales)[(int64_t)sm.lead[l] * a.num_kv_heads + head_of(hi)] = s;
+    }
+    __syncthreads();
+    walk([&](int kv, int e, int share) {
+      uint8_t* cache = static_cast<uint8_t*>(kv ? a.vc : a.kc);
+      const int l = e < n ? sm.row_lo[e] / kBlk : 0, off = e < n ? sm.row_lo[e] % kBlk : 0;
+      const int64_t block = (int64_t)sm.lead[l] * a.num_kv_heads;
+      if (!once) {
+        angles(kv, e);
+        if (share < nh) fetch(kv, e, head_of(share));
+      }
+      for (int hi = share; hi < nh; hi += sharing) {
+        if (!once) {
+          values(kv, e);
+          if (hi + sharing < nh) fetch(kv, e, head_of(hi + sharing));
+        }
+        if (e >= n) continue;
+        const float s = sm.now[kv][hi][l];
+        uint8_t* dst = cache + ((block + head_of(hi)) * kBlk + off) * a.head_dim;
+        const uint32_t bits = __float_as_uint(s);
+        if ((bits & 0x7fffffu) == 0u && bits >= (1u << 23) && bits < (254u << 23)) {
+          const float inv = __uint_as_float((254u << 23) - bits);  // x / 2^k = x 2^-k, exactly
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        if (un[k].has1) store_e4m3<V>(dst + un[k].o1, f[k]);
-        if (un[k].has2) store_e4m3<V>(dst + un[k].o2, f[k] + V);
-      }
-    }
-    // the blocks whose scale changed: the scale, and where it grew under
-    // rows that stay, those rows
-    bool grew = false;
-    float s_new = 0.f, s_old = 0.f;
-    if (lane < kBlk && !sm.dead[lane] && sm.lead[lane] >= 0) {
-      bool any = false;
-      for (int j = 0; j < kBlk; ++j) any = any || sm.win[lane][j] >= 0;
-      const bool fresh = sm.win[lane][0] >= 0;
-      const float need = block_scale(sm.top[buf][kv][lane]);
-      s_old = sm.old[buf][kv][lane];
-      s_new = fresh ? need : fmaxf(s_old, need);
-      grew = any && !fresh && s_new > s_old;
-      if (any && ht < 32) scales[(int64_t)sm.lead[lane] * a.num_kv_heads + head] = s_new;
-    }
-    uint32_t todo = __ballot_sync(0xffffffffu, grew);
-    while (todo != 0u) {
-      const int l = __ffs(todo) - 1;
-      todo &= todo - 1u;
-      const float ratio = __shfl_sync(0xffffffffu, s_old, l) / __shfl_sync(0xffffffffu, s_new, l);
-      const int chunks = a.head_dim / 16;
-      uint8_t* base = cache + ((int64_t)sm.lead[l] * a.num_kv_heads + head) * kBlk * a.head_dim;
-      for (int c = ht; c < kBlk * chunks; c += kThreads / 2) {
-        if (sm.win[l][c / chunks] >= 0) continue;
-        uint4* p = reinterpret_cast<uint4*>(base) + c;
-        float x[16];
-        load_widen<__nv_fp8_e4m3, 16>(reinterpret_cast<const __nv_fp8_e4m3*>(p), x);
+          for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] *= ratio;
-        store_e4m3<16>(reinterpret_cast<uint8_t*>(p), x);
+            for (int i = 0; i < 2 * V; ++i) f[k][i] *= inv;
+        } else if (s > 0.f) {  // a pool may hold scales that are no powers of two
+#pragma unroll
+          for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < 2 * V; ++i) f[k][i] = __fdiv_rn(f[k][i], s);
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          if (un[k].has1) store_e4m3<V>(dst + un[k].o1, f[k]);
+          if (un[k].has2) store_e4m3<V>(dst + un[k].o2, f[k] + V);
+        }
+      }
+    });
+    // blocks whose scale grew under rows that stay: those rows, a warp a block
+    for (int i0 = warp * 32; i0 < 2 * kHeads * kBlk; i0 += kThreads) {
+      const int i = i0 + lane, kvl = i / (kHeads * kBlk), hil = i / kBlk % kHeads, ll = i % kBlk;
+      const bool grew = hil < nh && sm.state[ll] != 0 && (sm.state[ll] & 1) == 0 && sm.now[kvl][hil][ll] > sm.old[kvl][hil][ll];
+      uint32_t todo = __ballot_sync(0xffffffffu, grew);
+      while (todo != 0u) {
+        const int j = i0 + __ffs(todo) - 1;
+        todo &= todo - 1u;
+        const int kv = j / (kHeads * kBlk), hi = j / kBlk % kHeads, l = j % kBlk;
+        const float ratio = sm.old[kv][hi][l] / sm.now[kv][hi][l];
+        const int chunks = a.head_dim / 16;
+        uint8_t* base = static_cast<uint8_t*>(kv ? a.vc : a.kc) +
+                        ((int64_t)sm.lead[l] * a.num_kv_heads + head_of(hi)) * kBlk * a.head_dim;
+        for (int c = lane; c < kBlk * chunks; c += 32) {
+          if ((sm.state[l] >> (c / chunks)) & 1) continue;
+          uint4* p = reinterpret_cast<uint4*>(base) + c;
+          float x[16];
+          load_widen<__nv_fp8_e4m3, 16>(reinterpret_cast<const __nv_fp8_e4m3*>(p), x);
+#pragma unroll
+          for (int k = 0; k < 16; ++k) x[k] *= ratio;
+          store_e4m3<16>(reinterpret_cast<uint8_t*>(p), x);
+        }
       }
     }
-    buf = next;
   }
 }
 
@@ -669,35 +741,51 @@ int row_layout(RopeArgs& a, int v) {
   return k;
 }
 
-template <typename T, int V, int K, int U, bool IL>
-cf_status launch_rows(const RopeArgs& a, int nrows, cudaStream_t stream) {
-  const int64_t rows = (int64_t)(32 >> a.lanes_log2) * U;
-  const int64_t items = (int64_t)a.num_tokens * ((nrows + rows - 1) / rows);
-  const int64_t want = (items + kWarps - 1) / kWarps, cap = (int64_t)sm_count() * 32;
-  rope_rows_kernel<T, V, K, U, IL><<<(unsigned)(want < cap ? want : cap), kThreads, 0, stream>>>(a);
-  return check_launch();
+// Whether every lane of a row has a unit that rotates.
+bool full_rows(const RopeArgs& a) { return a.rotary == a.head_dim && a.units == (1 << a.lanes_log2); }
+
+// CTAs for the row items of `heads` (a count per kind, 0 for none).
+unsigned row_ctas(const RopeArgs& a, int u, std::initializer_list<int> heads) {
+  const int rows = (32 >> a.lanes_log2) * u;
+  int64_t items = 0;
+  for (int h : heads) items += (h + rows - 1) / rows;
+  items *= a.num_tokens;
+  const int64_t want = (items + kWarps - 1) / kWarps, cap = (int64_t)sm_count() * 16;
+  return (unsigned)(want < cap ? want : cap);
 }
 
 template <typename T, int V, int K>
-cf_status launch_rows_of(const RopeArgs& a, bool interleaved, cudaStream_t stream) {
-  const int nrows = a.num_heads + a.num_kv_heads * (a.dest == kDense ? 1 : 2);
+cf_status launch_rows(const RopeArgs& a, bool interleaved, cudaStream_t stream) {
   constexpr int U = K == 1 ? 4 : 1;
-  return interleaved ? launch_rows<T, V, K, U, true>(a, nrows, stream)
-                     : launch_rows<T, V, K, U, false>(a, nrows, stream);
+  const unsigned grid = row_ctas(a, U, {a.num_heads, a.num_kv_heads, a.dest == kDense ? 0 : a.num_kv_heads});
+  if constexpr (K == 1) {
+    if (full_rows(a)) {
+      if (interleaved)
+        rope_rows_kernel<T, V, K, U, true, true><<<grid, kThreads, 0, stream>>>(a);
+      else
+        rope_rows_kernel<T, V, K, U, false, true><<<grid, kThreads, 0, stream>>>(a);
+      return check_launch();
+    }
+  }
+  if (interleaved)
+    rope_rows_kernel<T, V, K, U, true, false><<<grid, kThreads, 0, stream>>>(a);
+  else
+    rope_rows_kernel<T, V, K, U, false, false><<<grid, kThreads, 0, stream>>>(a);
+  return check_launch();
 }
 
 template <typename T>
 cf_status launch_rows_type(RopeArgs& a, bool interleaved, cudaStream_t stream) {
   const int v = vector_elems(a, sizeof(T));
   row_layout(a, v);
-  if (v == 16 / (int)sizeof(T)) return launch_rows_of<T, 16 / (int)sizeof(T), 1>(a, interleaved, stream);
+  if (v == 16 / (int)sizeof(T)) return launch_rows<T, 16 / (int)sizeof(T), 1>(a, interleaved, stream);
   if constexpr (sizeof(T) == 2)
-    if (v == 4) return launch_rows_of<T, 4, 1>(a, interleaved, stream);
-  return launch_rows_of<T, 1, 4>(a, interleaved, stream);
+    if (v == 4) return launch_rows<T, 4, 1>(a, interleaved, stream);
+  return launch_rows<T, 1, 4>(a, interleaved, stream);
 }
 
 template <typename T, int V, int K>
-cf_status launch_block_of(BlockArgs b, bool interleaved, cudaStream_t stream) {
+cf_status launch_block(BlockArgs b, bool interleaved, cudaStream_t stream) {
   const RopeArgs& a = b.r;
   const int windows = (a.num_tokens + kBlk - 1) / kBlk;
   // about four CTAs per SM: a CTA per (window, head) for decode steps, whole
@@ -706,19 +794,20 @@ cf_status launch_block_of(BlockArgs b, bool interleaved, cudaStream_t stream) {
   int split = (target + windows - 1) / windows;
   b.head_split = split < 1 ? 1 : (split > a.num_kv_heads ? a.num_kv_heads : split);
   b.kv_ctas = windows * b.head_split;
-  int64_t q_ctas = 0;
-  if (a.num_heads > 0) {
-    const int64_t rows = (int64_t)(32 >> a.lanes_log2) * (K == 1 ? 4 : 1);
-    const int64_t items = (int64_t)a.num_tokens * ((a.num_heads + rows - 1) / rows);
-    const int64_t cap = (int64_t)sm_count() * 32;
-    q_ctas = (items + kWarps - 1) / kWarps;
-    q_ctas = q_ctas < cap ? q_ctas : cap;
+  const unsigned grid = b.kv_ctas + (a.num_heads > 0 ? row_ctas(a, K == 1 ? 4 : 1, {a.num_heads}) : 0);
+  if constexpr (K == 1) {
+    if (full_rows(a)) {
+      if (interleaved)
+        rope_block_append_kernel<T, V, K, true, true><<<grid, kThreads, 0, stream>>>(b);
+      else
+        rope_block_append_kernel<T, V, K, false, true><<<grid, kThreads, 0, stream>>>(b);
+      return check_launch();
+    }
   }
-  const unsigned grid = (unsigned)(b.kv_ctas + q_ctas);
   if (interleaved)
-    rope_block_append_kernel<T, V, K, true><<<grid, kThreads, 0, stream>>>(b);
+    rope_block_append_kernel<T, V, K, true, false><<<grid, kThreads, 0, stream>>>(b);
   else
-    rope_block_append_kernel<T, V, K, false><<<grid, kThreads, 0, stream>>>(b);
+    rope_block_append_kernel<T, V, K, false, false><<<grid, kThreads, 0, stream>>>(b);
   return check_launch();
 }
 
@@ -726,10 +815,10 @@ template <typename T>
 cf_status launch_block_type(BlockArgs& b, bool interleaved, cudaStream_t stream) {
   const int v = vector_elems(b.r, sizeof(T));
   row_layout(b.r, v);
-  if (v == 16 / (int)sizeof(T)) return launch_block_of<T, 16 / (int)sizeof(T), 1>(b, interleaved, stream);
+  if (v == 16 / (int)sizeof(T)) return launch_block<T, 16 / (int)sizeof(T), 1>(b, interleaved, stream);
   if constexpr (sizeof(T) == 2)
-    if (v == 4) return launch_block_of<T, 4, 1>(b, interleaved, stream);
-  return launch_block_of<T, 1, 4>(b, interleaved, stream);
+    if (v == 4) return launch_block<T, 4, 1>(b, interleaved, stream);
+  return launch_block<T, 1, 4>(b, interleaved, stream);
 }
 
 RopeArgs rope_args(const cf_rope_params& p) {

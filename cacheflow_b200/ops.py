@@ -488,14 +488,15 @@ def reshape_and_cache_fp8_block(key, value, key_cache, value_cache, k_scales, v_
             or not key.is_cuda:
         raise _bad("key/value must be CUDA tensors [num_tokens, num_kv_heads, head_dim] of one dtype")
     T, Hkv, D = key.shape
-    dense = key.is_contiguous() and value.is_contiguous()
+    for t in (key, value):
+        if t.stride(2) != 1 and D > 1 or t.stride(1) != D and Hkv > 1:
+            raise _bad("key/value: a token's heads must be contiguous")
     _check_caches(key_cache, value_cache, key, torch.float8_e4m3fn, slot_mapping)
     _check_scales(k_scales, v_scales, key_cache)
-    if not dense:  # strided rows (slices of a fused projection)
-        key, value = key.contiguous(), value.contiguous()
     _on_device(lambda st: lib.cf_reshape_and_cache_fp8_block(
         _ptr(key), _ptr(value), _ptr(key_cache), _ptr(value_cache), _ptr(k_scales), _ptr(v_scales),
-        _ptr(slot_mapping), T, Hkv, D, key_cache.shape[2], key_cache.shape[0], dtype_code(key.dtype), st),
+        _ptr(slot_mapping), T, Hkv, D, key.stride(0), value.stride(0), key_cache.shape[2], key_cache.shape[0],
+        dtype_code(key.dtype), st),
         key, "cf_reshape_and_cache_fp8_block")
 
 

@@ -375,14 +375,16 @@ CF_API cf_status cf_rope_and_cache_fp8(const cf_rope_params* params, void* key_c
  * tokens count as consecutive calls of 16384).  The scale arrays move with
  * their blocks: cf_copy_blocks and the other block operators take them as
  * caches of block_size 1, head_dim 1, CF_F32.
- * key, value [num_tokens, num_kv_heads, head_dim], contiguous, of `dtype`
- * (CF_F32, CF_F16 or CF_BF16); head_dim a multiple of 16 up to 256;
+ * key, value [num_tokens, num_kv_heads, head_dim] of `dtype` (CF_F32, CF_F16
+ * or CF_BF16), tokens key_stride / value_stride elements apart, a token's
+ * heads contiguous; head_dim a multiple of 16 up to 256;
  * block_size 16; num_blocks > 0; caches 16-byte aligned. */
 CF_API cf_status cf_reshape_and_cache_fp8_block(const void* key, const void* value,
                                                 void* key_cache, void* value_cache,
                                                 float* k_scales, float* v_scales,
                                                 const int32_t* slot_mapping, int32_t num_tokens,
                                                 int32_t num_kv_heads, int32_t head_dim,
+                                                int64_t key_stride, int64_t value_stride,
                                                 int32_t block_size, int64_t num_blocks,
                                                 int32_t dtype, void* stream);
 
