@@ -18,6 +18,7 @@
 // Bound: HBM.  A row is read once and written once; the table row of a token
 // (R floats) is shared by all its heads.
 #include <initializer_list>
+#include <type_traits>
 
 #include "cf_device.cuh"
 #include "cf_internal.h"
@@ -49,6 +50,7 @@ struct RopeArgs {
   const void* k_w;
   int32_t w_f32;             // weights are f32 (else the rows' type)
   float eps;
+  float inv_dim;             // 1 / head_dim
   int32_t num_tokens, num_heads, num_kv_heads, head_dim, rotary, max_positions;
   int32_t dest;              // KDest
   void* kc;                  // [num_blocks, Hkv, block_size, D]
@@ -179,11 +181,39 @@ __device__ __forceinline__ Unit unit_of(const RopeArgs& a, int u) {
   return x;
 }
 
+// Two f32 in one register pair; the packed instructions do both at once and
+// round each as the scalar ones do.
+struct Pair {
+  uint64_t v;
+};
+__device__ __forceinline__ Pair pair(float lo, float hi) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(lo), "f"(hi));
+  return p;
+}
+__device__ __forceinline__ void split(Pair p, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p.v));
+}
+__device__ __forceinline__ Pair mul2(Pair x, Pair y) {
+  Pair p;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(x.v), "l"(y.v));
+  return p;
+}
+__device__ __forceinline__ Pair fma2(Pair x, Pair y, Pair z) {
+  Pair p;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p.v) : "l"(x.v), "l"(y.v), "l"(z.v));
+  return p;
+}
+
 // What a lane multiplies its pairs (a, b) with, weights and angles in one:
-//   a' = a ca - b sb,  b' = b cb + a sa   (columns that do not rotate: a ca, b cb)
+//   a' = a ca + b sb,  b' = b cb + a sa   (ca = ga cos, cb = gb cos, sa = ga
+//   sin, sb = -gb sin; columns that do not rotate: a ca, b cb)
+// Of V rotating pairs, as packed as the lane's vectors are: p1 holds what
+// multiplies the vectors themselves (ca then cb, or ca, cb, ca, ... when
+// interleaved), p2 what multiplies their partners.
 template <int V>
 struct Turn {
-  float ca[V], cb[V], sa[V], sb[V];
+  float p1[2 * V], p2[2 * V];
 };
 
 template <typename T, int V, int K, bool IL>
@@ -192,30 +222,38 @@ __device__ __forceinline__ void load_turn(const RopeArgs& a, const void* w, int 
   const float* row = a.positions != nullptr ? a.cos_sin + (size_t)pos * a.rotary : nullptr;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    float c[V], s[V], g[2 * V];
+    float c[V], s[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       c[i] = 1.f;
       s[i] = 0.f;
     }
-#pragma unroll
-    for (int i = 0; i < 2 * V; ++i) g[i] = 1.f;
     if (un[k].rot && row != nullptr) {
       const int i = (lane + (k << a.lanes_log2)) * V;
       load_f32<V>(row + i, c);
       load_f32<V>(row + a.rotary / 2 + i, s);
     }
-    if (w != nullptr) {
-      if (un[k].has1) load_weight<T, V>(a, w, un[k].o1, g);
-      if (un[k].has2) load_weight<T, V>(a, w, un[k].o2, g + V);
-    }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float ga = IL ? g[2 * i] : g[i], gb = IL ? g[2 * i + 1] : g[V + i];
-      tn[k].ca[i] = ga * c[i];
-      tn[k].cb[i] = gb * c[i];
-      tn[k].sa[i] = ga * s[i];
-      tn[k].sb[i] = gb * s[i];
+      const int ia = IL ? 2 * i : i, ib = IL ? 2 * i + 1 : V + i;
+      tn[k].p1[ia] = tn[k].p1[ib] = c[i];
+      tn[k].p2[ia] = -s[i];
+      tn[k].p2[ib] = s[i];
+    }
+    if (w != nullptr) {  // p1 has its own column's weight, p2 the partner's
+      float g[2 * V];
+#pragma unroll
+      for (int i = 0; i < 2 * V; ++i) g[i] = 1.f;
+      if (un[k].has1) load_weight<T, V>(a, w, un[k].o1, g);
+      if (un[k].has2) load_weight<T, V>(a, w, un[k].o2, g + V);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int ia = IL ? 2 * i : i, ib = IL ? 2 * i + 1 : V + i;
+        tn[k].p1[ia] *= g[ia];
+        tn[k].p1[ib] *= g[ib];
+        tn[k].p2[ia] *= g[ib];
+        tn[k].p2[ib] *= g[ia];
+      }
     }
   }
 }
@@ -233,35 +271,59 @@ __device__ __forceinline__ void norm_turn(const RopeArgs& a, float (&f)[K][2 * V
                                           const Turn<V> (&tn)[K]) {
   float rs = 1.f;
   if (norm) {
-    float s0 = 0.f, s1 = 0.f;  // two chains
+    float ss = 0.f;
+    if constexpr (V % 2 == 0) {
+      Pair s0 = pair(0.f, 0.f), s1 = s0;  // four chains
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+      for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        s0 = fmaf(f[k][i], f[k][i], s0);
-        s1 = fmaf(f[k][V + i], f[k][V + i], s1);
-      }
-    rs = rsqrtf(row_sum(s0 + s1, a.lanes_log2) / (float)a.head_dim + a.eps);
+        for (int i = 0; i < V; i += 2) {
+          const Pair x = pair(f[k][i], f[k][i + 1]), y = pair(f[k][V + i], f[k][V + i + 1]);
+          s0 = fma2(x, x, s0);
+          s1 = fma2(y, y, s1);
+        }
+      float a0, a1, b0, b1;
+      split(s0, a0, a1);
+      split(s1, b0, b1);
+      ss = (a0 + a1) + (b0 + b1);
+    } else {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < 2 * V; ++i) ss = fmaf(f[k][i], f[k][i], ss);
+    }
+    rs = rsqrtf(fmaf(row_sum(ss, a.lanes_log2), a.inv_dim, a.eps));
   }
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const Turn<V>& t = tn[k];
+    if (!un[k].rot) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int ia = IL ? 2 * i : i, ib = IL ? 2 * i + 1 : V + i;
-      float& x = f[k][ia];
-      float& y = f[k][ib];
-      const float xa = x, yb = y;
-      if (un[k].rot) {
-        x = fmaf(xa, t.ca[i], -(yb * t.sb[i]));
-        y = fmaf(yb, t.cb[i], xa * t.sa[i]);
-      } else {
-        x = xa * t.ca[i];
-        y = yb * t.cb[i];
+      for (int i = 0; i < 2 * V; ++i) f[k][i] = f[k][i] * t.p1[i] * rs;
+    } else if constexpr (V % 2 == 0) {
+      const Pair r = pair(rs, rs);
+#pragma unroll
+      for (int i = 0; i < V; i += 2) {
+        // two neighbouring columns each, and their partners'
+        const int j = IL ? 2 * i : i, j2 = IL ? 2 * i + 2 : V + i;
+        const Pair x = pair(f[k][j], f[k][j + 1]), y = pair(f[k][j2], f[k][j2 + 1]);
+        const Pair xp = IL ? pair(f[k][j + 1], f[k][j]) : y, yp = IL ? pair(f[k][j2 + 1], f[k][j2]) : x;
+        Pair u = fma2(x, pair(t.p1[j], t.p1[j + 1]), mul2(xp, pair(t.p2[j], t.p2[j + 1])));
+        Pair v = fma2(y, pair(t.p1[j2], t.p1[j2 + 1]), mul2(yp, pair(t.p2[j2], t.p2[j2 + 1])));
+        if (norm) {
+          u = mul2(u, r);
+          v = mul2(v, r);
+        }
+        split(u, f[k][j], f[k][j + 1]);
+        split(v, f[k][j2], f[k][j2 + 1]);
       }
-      if (norm) {
-        x *= rs;
-        y *= rs;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int ia = IL ? 2 * i : i, ib = IL ? 2 * i + 1 : V + i;
+        const float x = f[k][ia], y = f[k][ib];
+        f[k][ia] = fmaf(x, t.p1[ia], y * t.p2[ia]) * rs;
+        f[k][ib] = fmaf(y, t.p1[ib], x * t.p2[ib]) * rs;
       }
     }
   }
@@ -270,11 +332,29 @@ __device__ __forceinline__ void norm_turn(const RopeArgs& a, float (&f)[K][2 * V
 // ---------------------------------------------------------------------------
 // Row items.  A warp takes 32 / lanes heads of one token and one kind (Q, K
 // or V) at a time, U times over: the token's angles and the kind's weights are
-// loaded and multiplied once for all of them, every branch on the kind is the
-// whole warp's, and the 2U loads per lane are in flight together.
+// loaded and multiplied once for all of them, and every branch on the kind is
+// the whole warp's.  A lane copies its vectors of the next item into its own
+// slots of shared memory (cp.async, which only the lane itself waits for)
+// while it works on this one, and has the position and slot after that on
+// their way.
 // ---------------------------------------------------------------------------
+constexpr int kItemStages = 2;
+template <typename T, int V, int K, int U>
+constexpr int kItemBytes = K == 1 ? U * 2 * 32 * V * (int)sizeof(T) : 0;  // of a warp and stage
+
+// One vector into shared memory; zeros where there is none.
+template <int kBytes>
+__device__ __forceinline__ void copy_or_zero(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(kBytes),
+               "r"(there ? kBytes : 0)
+               : "memory");
+}
+
 template <typename T, int V, int K, int U, bool IL, bool kFull>
-__device__ __forceinline__ void row_items(const RopeArgs& a, int64_t warp, int64_t num_warps, bool with_kv) {
+__device__ __forceinline__ void row_items(const RopeArgs& a, int64_t warp, int64_t num_warps, bool with_kv,
+                                          uint8_t* buffer) {
+  constexpr bool kPipe = K == 1;  // (a lane of one-element vectors loads where it uses them)
+  constexpr int VB = V * (int)sizeof(T);
   const int lane = threadIdx.x & 31;
   const int sub = lane & ((1 << a.lanes_log2) - 1);
   const int per_warp = 32 >> a.lanes_log2;
@@ -287,106 +367,165 @@ __device__ __forceinline__ void row_items(const RopeArgs& a, int64_t warp, int64
   for (int k = 0; k < K; ++k) un[k] = unit_of<V, IL, kFull>(a, sub + (k << a.lanes_log2));
 
   // item = t * per_token + c, advanced without a division
-  int64_t t = warp / per_token;
-  int c = (int)(warp - t * per_token);
+  struct Item {
+    int64_t t;
+    int c, pos, slot;
+  };
   const int64_t dt = num_warps / per_token;
   const int dc = (int)(num_warps - dt * per_token);
-  for (; t < a.num_tokens; t += dt, c += dc) {
-    if (c >= per_token) {
-      c -= per_token;
-      if (++t >= a.num_tokens) break;
+  auto look = [&](Item& x) {
+    x.pos = a.positions != nullptr && x.t < a.num_tokens ? a.positions[x.t] : 0;
+    x.slot = a.slots != nullptr && x.t < a.num_tokens ? a.slots[x.t] : -1;
+  };
+  auto advance = [&](Item x) {
+    x.t += dt;
+    x.c += dc;
+    if (x.c >= per_token) {
+      x.c -= per_token;
+      ++x.t;
     }
-    const int kind = c < nq ? 0 : (c < nq + nk ? 1 : 2);
-    const int heads = kind == 0 ? a.num_heads : a.num_kv_heads;
-    const int head0 = (kind == 0 ? c : kind == 1 ? c - nq : c - nq - nk) * per_warp * U + grp;
-    const void* base = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-    const int64_t ts = kind == 0 ? a.q_ts : kind == 1 ? a.k_ts : a.v_ts;
-    const int64_t hs = kind == 0 ? a.q_hs : kind == 1 ? a.k_hs : a.v_hs;
-    int pos = 0;
-    if (a.positions != nullptr) pos = a.positions[t];
-    int64_t slot = -1;
-    if (a.slots != nullptr && kind > 0) slot = a.slots[t];
-    const T* src = static_cast<const T*>(base) + t * ts + head0 * hs;
-    Raw<T, V> raw[U][K][2];
+    look(x);
+    return x;
+  };
+  auto kind_of = [&](int c) { return c < nq ? 0 : (c < nq + nk ? 1 : 2); };
+  auto heads_of = [&](int kind) { return kind == 0 ? a.num_heads : a.num_kv_heads; };
+  auto head_of = [&](int c, int kind) { return (kind == 0 ? c : kind == 1 ? c - nq : c - nq - nk) * per_warp * U + grp; };
+  auto stride_of = [&](int kind) { return kind == 0 ? a.q_hs : kind == 1 ? a.k_hs : a.v_hs; };
+  auto row_of = [&](const Item& x, int kind, int head) {
+    const T* base = static_cast<const T*>(kind == 0 ? a.q : kind == 1 ? a.k : a.v);
+    return base + x.t * (kind == 0 ? a.q_ts : kind == 1 ? a.k_ts : a.v_ts) + head * stride_of(kind);
+  };
+  uint8_t* mine = buffer + lane * VB;  // [stage][u][2][lane]
+  auto copy = [&](const Item& x, int stage) {
+    if (x.t < a.num_tokens) {
+      const int kind = kind_of(x.c), heads = heads_of(kind), head0 = head_of(x.c, kind);
+      const int64_t hs = stride_of(kind);
+      const T* p = row_of(x, kind, head0);
+      const uint32_t dst = smem_addr(mine) + stage * kItemBytes<T, V, K, U>;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (head0 + u * per_warp < heads) {
-        const T* p = src + (int64_t)(u * per_warp) * hs;
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          if (un[k].has1) raw[u][k][0] = *reinterpret_cast<const Raw<T, V>*>(p + un[k].o1);
-          if (un[k].has2) raw[u][k][1] = *reinterpret_cast<const Raw<T, V>*>(p + un[k].o2);
-        }
+      for (int u = 0; u < U; ++u) {
+        // where a row or a vector does not exist, nothing is read: the address is the base's
+        const bool there = head0 + u * per_warp < heads;
+        const T* r = there ? p + (int64_t)(u * per_warp) * hs : static_cast<const T*>(a.k);
+        copy_or_zero<VB>(dst + (2 * u) * 32 * VB, r + (there && un[0].has1 ? un[0].o1 : 0), there && un[0].has1);
+        copy_or_zero<VB>(dst + (2 * u + 1) * 32 * VB, r + (there && un[0].has2 ? un[0].o2 : 0), there && un[0].has2);
       }
     }
+    cp_async_commit();
+  };
+
+  Item now;
+  now.t = warp / per_token;
+  now.c = (int)(warp - now.t * per_token);
+  look(now);
+  Item next = advance(now);
+  if constexpr (kPipe) copy(now, 0);
+  for (int stage = 0; now.t < a.num_tokens; stage ^= 1) {
+    if constexpr (kPipe) copy(next, stage ^ 1);
+    const Item x = now;
+    now = next;
+    next = advance(next);
+    if constexpr (kPipe) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    const int kind = kind_of(x.c), heads = heads_of(kind), head0 = head_of(x.c, kind);
     if (a.positions != nullptr) {
-      if (pos >= a.max_positions && lane == 0) rope_error(CF_DEVERR_POSITION);
-      if (pos < 0 || pos >= a.max_positions) continue;  // a padding token, or one without angles: left out whole
+      if (x.pos >= a.max_positions && lane == 0) rope_error(CF_DEVERR_POSITION);
+      if (x.pos < 0 || x.pos >= a.max_positions) continue;  // a padding token, or one without angles: left out whole
     }
     const bool cached = kind > 0 && a.dest != kDense;
     if (cached) {
-      if (slot >= a.num_slots && lane == 0) rope_error(CF_DEVERR_SLOT);
-      if (slot < 0 || slot >= a.num_slots) continue;  // a padding row: nothing is appended
+      if (x.slot >= a.num_slots && lane == 0) rope_error(CF_DEVERR_SLOT);
+      if (x.slot < 0 || x.slot >= a.num_slots) continue;  // a padding row: nothing is appended
     }
     const void* w = kind == 0 ? a.q_w : kind == 1 ? a.k_w : nullptr;
-    Turn<V> tn[K];
-    if (kind < 2) load_turn<T, V, K, IL>(a, w, pos, sub, un, tn);
     // the rows' destination, element strides as the source's
-    const int64_t blk = cached ? slot / a.block_size : 0;
+    const uint32_t blk = cached ? (uint32_t)x.slot / (uint32_t)a.block_size : 0u;
+    const uint32_t off = cached ? (uint32_t)x.slot - blk * (uint32_t)a.block_size : 0u;
     const int64_t dhs = cached ? (int64_t)a.block_size * a.head_dim : kind == 0 ? a.qo_hs : a.ko_hs;
-    const int64_t d0 = cached ? (blk * a.num_kv_heads * a.block_size + (slot - blk * a.block_size)) * a.head_dim
-                              : kind == 0 ? t * a.qo_ts : t * a.ko_ts;
+    const int64_t row0 = (cached ? ((int64_t)blk * a.num_kv_heads * a.block_size + off) * a.head_dim
+                                 : kind == 0 ? x.t * a.qo_ts : x.t * a.ko_ts) + head0 * dhs;
     void* dbase = cached ? (kind == 1 ? a.kc : a.vc) : kind == 0 ? a.q_out : a.k_out;
-    const bool fp8 = cached && a.dest == kCacheFp8;
     const float sc = kind == 1 ? a.k_scale : a.v_scale;
+    const int64_t hs = stride_of(kind);
+    const T* src = row_of(x, kind, head0);
+    // kTurn: normed and rotated; kQuant: stored as e4m3; neither: moved as
+    // they are, bit for bit.  kWhole: every row of the item exists.
+    auto finish = [&](auto turn, auto quant, auto whole) {
+      constexpr bool kTurn = decltype(turn)::value, kQuant = decltype(quant)::value, kWhole = decltype(whole)::value;
+      Turn<V> tn[K];
+      if (kTurn) load_turn<T, V, K, IL>(a, w, x.pos, sub, un, tn);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int head = head0 + u * per_warp;
-      if (u > 0 && head - grp >= heads) break;  // for the whole warp
-      const bool valid = head < heads;
-      float f[K][2 * V];
-      if (kind < 2 || fp8) {
+      for (int u = 0; u < U; ++u) {
+        if (!kWhole && u > 0 && head0 - grp + u * per_warp >= heads) break;  // for the whole warp
+        const bool there = kWhole || head0 + u * per_warp < heads;
+        Raw<T, V> raw[K][2];
+        if constexpr (kPipe) {
+          const uint8_t* p = mine + stage * kItemBytes<T, V, K, U> + 2 * u * 32 * VB;
+          raw[0][0] = *reinterpret_cast<const Raw<T, V>*>(p);
+          raw[0][1] = *reinterpret_cast<const Raw<T, V>*>(p + 32 * VB);
+        } else {
+          const T* p = src + (int64_t)(u * per_warp) * hs;
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-          if (!kFull || !valid) {
-#pragma unroll
-            for (int i = 0; i < 2 * V; ++i) f[k][i] = 0.f;
+          for (int k = 0; k < K; ++k) {
+            raw[k][0] = raw[k][1] = Raw<T, V>{};
+            if (there && un[k].has1) raw[k][0] = *reinterpret_cast<const Raw<T, V>*>(p + un[k].o1);
+            if (there && un[k].has2) raw[k][1] = *reinterpret_cast<const Raw<T, V>*>(p + un[k].o2);
           }
-          if (valid && un[k].has1) unpack<T, V>(raw[u][k][0], f[k]);
-          if (valid && un[k].has2) unpack<T, V>(raw[u][k][1], f[k] + V);
         }
-        if (kind < 2) norm_turn<V, K, IL>(a, f, w != nullptr, un, tn);
+        float f[K][2 * V];
+        if (kTurn || kQuant) {
+#pragma unroll
+          for (int k = 0; k < K; ++k) {
+            unpack<T, V>(raw[k][0], f[k]);
+            unpack<T, V>(raw[k][1], f[k] + V);
+          }
+        }
+        if (kTurn) norm_turn<V, K, IL>(a, f, w != nullptr, un, tn);
+        if (!there) continue;
+        const int64_t row = row0 + (int64_t)(u * per_warp) * dhs;
+        if (kQuant) {
+          uint8_t* dst = static_cast<uint8_t*>(dbase) + row;
+#pragma unroll
+          for (int k = 0; k < K; ++k) {
+#pragma unroll
+            for (int i = 0; i < 2 * V; ++i) f[k][i] = __fdiv_rn(f[k][i], sc);
+            if (un[k].has1) store_e4m3<V>(dst + un[k].o1, f[k]);
+            if (un[k].has2) store_e4m3<V>(dst + un[k].o2, f[k] + V);
+          }
+        } else {
+          T* dst = static_cast<T*>(dbase) + row;
+#pragma unroll
+          for (int k = 0; k < K; ++k) {
+            if (un[k].has1) *reinterpret_cast<Raw<T, V>*>(dst + un[k].o1) = kTurn ? pack<T, V>(f[k]) : raw[k][0];
+            if (un[k].has2) *reinterpret_cast<Raw<T, V>*>(dst + un[k].o2) = kTurn ? pack<T, V>(f[k] + V) : raw[k][1];
+          }
+        }
       }
-      if (!valid) continue;
-      const int64_t row = d0 + head * dhs;
-      if (fp8) {
-        uint8_t* dst = static_cast<uint8_t*>(dbase) + row;
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-#pragma unroll
-          for (int i = 0; i < 2 * V; ++i) f[k][i] = __fdiv_rn(f[k][i], sc);
-          if (un[k].has1) store_e4m3<V>(dst + un[k].o1, f[k]);
-          if (un[k].has2) store_e4m3<V>(dst + un[k].o2, f[k] + V);
-        }
-      } else {
-        T* dst = static_cast<T*>(dbase) + row;
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          // V is moved as it is, bit for bit
-          if (un[k].has1)
-            *reinterpret_cast<Raw<T, V>*>(dst + un[k].o1) = kind == 2 ? raw[u][k][0] : pack<T, V>(f[k]);
-          if (un[k].has2)
-            *reinterpret_cast<Raw<T, V>*>(dst + un[k].o2) = kind == 2 ? raw[u][k][1] : pack<T, V>(f[k] + V);
-        }
-      }
-    }
+    };
+    using Y = std::true_type;
+    using N = std::false_type;
+    const bool fp8 = cached && a.dest == kCacheFp8;
+    if (kind < 2 && !fp8)
+      head0 - grp + U * per_warp <= heads ? finish(Y{}, N{}, Y{}) : finish(Y{}, N{}, N{});
+    else if (kind < 2)
+      finish(Y{}, Y{}, N{});
+    else if (fp8)
+      finish(N{}, Y{}, N{});
+    else
+      finish(N{}, N{}, N{});
   }
+  if constexpr (kPipe) cp_async_wait_all();
 }
 
+constexpr int kRowThreads = 128;
+constexpr int kRowWarps = kRowThreads / 32;
+
 template <typename T, int V, int K, int U, bool IL, bool kFull>
-__global__ void __launch_bounds__(kThreads) rope_rows_kernel(const __grid_constant__ RopeArgs a) {
-  row_items<T, V, K, U, IL, kFull>(a, (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5), (int64_t)gridDim.x * kWarps,
-                                   true);
+__global__ void __launch_bounds__(kRowThreads) rope_rows_kernel(const __grid_constant__ RopeArgs a) {
+  constexpr int kArea = kItemStages * kItemBytes<T, V, K, U>;
+  __shared__ __align__(16) uint8_t buffer[kRowWarps * kArea + 16];
+  const int warp = threadIdx.x >> 5;
+  row_items<T, V, K, U, IL, kFull>(a, (int64_t)blockIdx.x * kRowWarps + warp, (int64_t)gridDim.x * kRowWarps, true,
+                                   buffer + warp * kArea);
 }
 
 // ---------------------------------------------------------------------------
@@ -453,12 +592,18 @@ __device__ __forceinline__ float block_scale(uint32_t bits) {
 template <typename T, int V, int K, bool IL, bool kFull>
 __global__ void __launch_bounds__(kThreads) rope_block_append_kernel(const __grid_constant__ BlockArgs b) {
   const RopeArgs& a = b.r;
+  constexpr int U = K == 1 ? 2 : 1, kArea = kItemStages * kItemBytes<T, V, K, U>;
+  __shared__ union {
+    BlockSmem sm;
+    __align__(16) uint8_t buffer[kWarps * kArea + 16];
+  } smem;
   if ((int)blockIdx.x >= b.kv_ctas) {
-    row_items<T, V, K, K == 1 ? 4 : 1, IL, kFull>(a, (int64_t)(blockIdx.x - b.kv_ctas) * kWarps + (threadIdx.x >> 5),
-                                                  (int64_t)(gridDim.x - b.kv_ctas) * kWarps, false);
+    const int warp = threadIdx.x >> 5;
+    row_items<T, V, K, U, IL, kFull>(a, (int64_t)(blockIdx.x - b.kv_ctas) * kWarps + warp,
+                                     (int64_t)(gridDim.x - b.kv_ctas) * kWarps, false, smem.buffer + warp * kArea);
     return;
   }
-  __shared__ BlockSmem sm;
+  BlockSmem& sm = smem.sm;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int window = blockIdx.x / b.head_split;
   const int w0 = window * kBlk;
@@ -563,6 +708,10 @@ __global__ void __launch_bounds__(kThreads) rope_block_append_kernel(const __gri
   Raw<T, V> raw[K][2];
   Turn<V> tn[K];
   float f[K][2 * V];
+  auto clear = [&]() {  // what no row or unit fills stays zero
+#pragma unroll
+    for (int k = 0; k < K; ++k) raw[k][0] = raw[k][1] = Raw<T, V>{};
+  };
   auto fetch = [&](int kv, int e, int head) {  // row e of the list
     if (e < n) {
       const T* p = static_cast<const T*>(kv ? a.v : a.k) + (int64_t)sm.row_tok[e] * (kv ? a.v_ts : a.k_ts) +
@@ -579,13 +728,11 @@ __global__ void __launch_bounds__(kThreads) rope_block_append_kernel(const __gri
     if (turns(kv) && e < n)
       load_turn<T, V, K, IL>(a, a.k_w, a.positions != nullptr ? a.positions[sm.row_tok[e]] : 0, sub, un, tn);
   };
-  auto values = [&](int kv, int e) {  // what was fetched, normed and turned
+  auto values = [&](int kv) {  // what was fetched, normed and turned
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-#pragma unroll
-      for (int i = 0; i < 2 * V; ++i) f[k][i] = 0.f;
-      if (e < n && un[k].has1) unpack<T, V>(raw[k][0], f[k]);
-      if (e < n && un[k].has2) unpack<T, V>(raw[k][1], f[k] + V);
+      unpack<T, V>(raw[k][0], f[k]);
+      unpack<T, V>(raw[k][1], f[k] + V);
     }
     if (turns(kv)) norm_turn<V, K, IL>(a, f, a.k_w != nullptr, un, tn);
   };
@@ -612,10 +759,11 @@ __global__ void __launch_bounds__(kThreads) rope_block_append_kernel(const __gri
       }
     };
     walk([&](int kv, int e, int share) {
+      clear();
       angles(kv, e);
       if (share < nh) fetch(kv, e, head_of(share));
       for (int hi = share; hi < nh; hi += sharing) {
-        values(kv, e);
+        values(kv);
         if (hi + sharing < nh) fetch(kv, e, head_of(hi + sharing));
         float top = 0.f;
 #pragma unroll
@@ -644,12 +792,13 @@ __global__ void __launch_bounds__(kThreads) rope_block_append_kernel(const __gri
       const int l = e < n ? sm.row_lo[e] / kBlk : 0, off = e < n ? sm.row_lo[e] % kBlk : 0;
       const int64_t block = (int64_t)sm.lead[l] * a.num_kv_heads;
       if (!once) {
+        clear();
         angles(kv, e);
         if (share < nh) fetch(kv, e, head_of(share));
       }
       for (int hi = share; hi < nh; hi += sharing) {
         if (!once) {
-          values(kv, e);
+          values(kv);
           if (hi + sharing < nh) fetch(kv, e, head_of(hi + sharing));
         }
         if (e >= n) continue;
@@ -744,34 +893,50 @@ int row_layout(RopeArgs& a, int v) {
 // Whether every lane of a row has a unit that rotates.
 bool full_rows(const RopeArgs& a) { return a.rotary == a.head_dim && a.units == (1 << a.lanes_log2); }
 
-// CTAs for the row items of `heads` (a count per kind, 0 for none).
-unsigned row_ctas(const RopeArgs& a, int u, std::initializer_list<int> heads) {
+// CTAs of `warps` warps for the row items of `heads` (a count per kind, 0 for none).
+unsigned row_ctas(const RopeArgs& a, int u, int warps, std::initializer_list<int> heads) {
   const int rows = (32 >> a.lanes_log2) * u;
   int64_t items = 0;
   for (int h : heads) items += (h + rows - 1) / rows;
   items *= a.num_tokens;
-  const int64_t want = (items + kWarps - 1) / kWarps, cap = (int64_t)sm_count() * 16;
+  const int64_t want = (items + warps - 1) / warps, cap = (int64_t)sm_count() * 64 / warps;
   return (unsigned)(want < cap ? want : cap);
 }
 
-template <typename T, int V, int K>
-cf_status launch_rows(const RopeArgs& a, bool interleaved, cudaStream_t stream) {
-  constexpr int U = K == 1 ? 4 : 1;
-  const unsigned grid = row_ctas(a, U, {a.num_heads, a.num_kv_heads, a.dest == kDense ? 0 : a.num_kv_heads});
+template <typename T, int V, int K, int U>
+cf_status launch_rows_u(const RopeArgs& a, bool interleaved, unsigned grid, cudaStream_t stream) {
   if constexpr (K == 1) {
     if (full_rows(a)) {
       if (interleaved)
-        rope_rows_kernel<T, V, K, U, true, true><<<grid, kThreads, 0, stream>>>(a);
+        rope_rows_kernel<T, V, K, U, true, true><<<grid, kRowThreads, 0, stream>>>(a);
       else
-        rope_rows_kernel<T, V, K, U, false, true><<<grid, kThreads, 0, stream>>>(a);
+        rope_rows_kernel<T, V, K, U, false, true><<<grid, kRowThreads, 0, stream>>>(a);
       return check_launch();
     }
   }
   if (interleaved)
-    rope_rows_kernel<T, V, K, U, true, false><<<grid, kThreads, 0, stream>>>(a);
+    rope_rows_kernel<T, V, K, U, true, false><<<grid, kRowThreads, 0, stream>>>(a);
   else
-    rope_rows_kernel<T, V, K, U, false, false><<<grid, kThreads, 0, stream>>>(a);
+    rope_rows_kernel<T, V, K, U, false, false><<<grid, kRowThreads, 0, stream>>>(a);
   return check_launch();
+}
+
+template <typename T, int V, int K>
+cf_status launch_rows(const RopeArgs& a, bool interleaved, cudaStream_t stream) {
+  auto ctas = [&](int u) {
+    return row_ctas(a, u, kRowWarps, {a.num_heads, a.num_kv_heads, a.dest == kDense ? 0 : a.num_kv_heads});
+  };
+  if constexpr (K == 1) {
+    // Heads per lane group and item: four 16-bit rows (8192 tokens of 64 / 8
+    // heads 64 us, 77 with two), two f32 ones (4095 tokens of 32 / 32 heads 29
+    // us, 32 with four), one where a call has few items (a token of 32 / 8
+    // heads 3.8 us, 4.3 with four).
+    constexpr int U = sizeof(T) == 4 ? 2 : 4;
+    const unsigned grid = ctas(U);
+    if (grid < (unsigned)sm_count()) return launch_rows_u<T, V, K, 1>(a, interleaved, ctas(1), stream);
+    return launch_rows_u<T, V, K, U>(a, interleaved, grid, stream);
+  }
+  return launch_rows_u<T, V, K, 1>(a, interleaved, ctas(1), stream);
 }
 
 template <typename T>
@@ -794,7 +959,7 @@ cf_status launch_block(BlockArgs b, bool interleaved, cudaStream_t stream) {
   int split = (target + windows - 1) / windows;
   b.head_split = split < 1 ? 1 : (split > a.num_kv_heads ? a.num_kv_heads : split);
   b.kv_ctas = windows * b.head_split;
-  const unsigned grid = b.kv_ctas + (a.num_heads > 0 ? row_ctas(a, K == 1 ? 4 : 1, {a.num_heads}) : 0);
+  const unsigned grid = b.kv_ctas + (a.num_heads > 0 ? row_ctas(a, K == 1 ? 2 : 1, kWarps, {a.num_heads}) : 0);
   if constexpr (K == 1) {
     if (full_rows(a)) {
       if (interleaved)
@@ -839,6 +1004,7 @@ RopeArgs rope_args(const cf_rope_params& p) {
   a.k_w = p.key_weight;
   a.w_f32 = p.weight_dtype == CF_F32;
   a.eps = p.eps;
+  a.inv_dim = 1.f / (float)p.head_dim;
   a.num_tokens = p.num_tokens;
   a.num_heads = p.num_heads;
   a.num_kv_heads = p.num_kv_heads;

@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import numpy as np
 import torch
@@ -335,13 +336,16 @@ def _bad(what: str) -> CacheFlowError:
     return CacheFlowError(_lib.CF_ERR_INVALID_ARGUMENT, what)
 
 
-def _on_device(call, t: torch.Tensor, what: str) -> None:
-    """Runs call(stream) on t's device and its current stream; raises on a status."""
-    if t.device.index == torch.cuda.current_device():
-        check(call(_stream(t)), what)
+def _call(fn, device: int, what: str, *args) -> None:
+    """fn(*args, stream) on `device` and its current stream; raises on a status.  Every microsecond here is one of
+    a small call's, so the raw stream is asked for and the device only changed where it is another one."""
+    if device == torch.cuda.current_device():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
-        with torch.cuda.device(t.device):
-            check(call(_stream(t)), what)
+        with torch.cuda.device(device):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if status != _lib.CF_OK:
+        check(status, what)
 
 
 def rope_table(max_positions: int, rotary_dim: int, base: float = 10000.0, device="cuda") -> torch.Tensor:
@@ -355,47 +359,67 @@ def rope_table(max_positions: int, rotary_dim: int, base: float = 10000.0, devic
     return torch.cat([a.cos(), a.sin()], dim=1).to(torch.float32)
 
 
+# cf_rope_params, packed in one go: nine pointers, five {token, head} strides,
+# the sizes, eps, interleaved and the two types.
+_ROPE_PARAMS = struct.Struct("=9Q10q6if3i")
+assert _ROPE_PARAMS.size == ctypes.sizeof(_lib.RopeParams)
+
+
+# cf_paged_attention_params: six pointers, the scale, seven sizes, num_blocks
+# (8-byte aligned), the type and the tail's padding.
+_ATTENTION_PARAMS = struct.Struct("=6Qf7iqi4x")
+assert _ATTENTION_PARAMS.size == ctypes.sizeof(AttentionParams)
+
+
+def _rows(name, t, shape, dt, dev):
+    """(pointer, token stride, head stride) of [tokens, heads, head_dim] rows."""
+    if t.shape != shape or t.dtype != dt or t.get_device() != dev:
+        raise _bad(f"{name} must be {dt} of shape {tuple(shape)} on cuda:{dev}")
+    s0, s1, s2 = t.stride()
+    if s2 != 1 and shape[2] > 1:
+        raise _bad(f"{name}: the last dimension must be contiguous")
+    return t.data_ptr(), s0, s1
+
+
 def _rope_params(q_out, query, key, positions, cos_sin, q_weight, k_weight, eps, interleaved, value=None,
                  k_out=None):
-    if query.dim() != 3 or key.dim() != 3:
-        raise _bad("query/key must be [num_tokens, heads, head_dim]")
-    T, H, D = query.shape
-    Hkv = key.shape[1]
-    dt, dev = query.dtype, query.device
-    if not query.is_cuda:
-        raise _bad("query must be a CUDA tensor")
-    p = _lib.RopeParams()
-    for name, t, shape in (("query", query, (T, H, D)), ("key", key, (T, Hkv, D)), ("value", value, (T, Hkv, D)),
-                           ("query_out", q_out, (T, H, D)), ("key_out", k_out, (T, Hkv, D))):
-        if t is None:
-            continue
-        if tuple(t.shape) != shape or t.dtype != dt or t.device != dev:
-            raise _bad(f"{name} must be {dt} of shape {shape} on {dev}")
-        st = t.stride()
-        if st[2] != 1 and D > 1:
-            raise _bad(f"{name}: the last dimension must be contiguous")
-        setattr(p, name, t.data_ptr())
-        getattr(p, name + "_stride")[:] = st[:2]
-    if positions.dtype != torch.int32 or positions.shape != (T,) or not positions.is_contiguous() \
-            or positions.device != dev:
-        raise _bad(f"positions must be contiguous int32 of shape ({T},) on {dev}")
-    if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous() or cos_sin.device != dev:
-        raise _bad(f"cos_sin must be contiguous float32 [max_positions, rotary_dim] on {dev}")
-    p.positions, p.cos_sin = positions.data_ptr(), cos_sin.data_ptr()
-    p.dtype = p.weight_dtype = dtype_code(dt)
-    given = [w for w in (q_weight, k_weight) if w is not None]
-    for w in given:
-        if w.shape != (D,) or not w.is_contiguous() or w.device != dev or w.dtype not in (dt, torch.float32) \
-                or w.dtype != given[0].dtype:
-            raise _bad(f"norm weights must be contiguous ({D},) on {dev}, both float32 or both {dt}")
-    if given:
-        p.weight_dtype = dtype_code(given[0].dtype)
-        p.query_weight, p.key_weight = _ptr(q_weight), _ptr(k_weight)
-    p.num_tokens, p.num_heads, p.num_kv_heads, p.head_dim = T, H, Hkv, D
-    p.max_positions, p.rotary_dim = cos_sin.shape
-    p.eps = float(eps)
-    p.interleaved = 1 if interleaved else 0
-    return p
+    qs, ks = query.shape, key.shape
+    if len(qs) != 3 or len(ks) != 3 or not query.is_cuda:
+        raise _bad("query/key must be CUDA tensors [num_tokens, heads, head_dim]")
+    T, H, D = qs
+    dt, dev = query.dtype, query.get_device()
+    if ks[0] != T or ks[2] != D:
+        raise _bad("query and key must have the same tokens and head_dim")
+    q, q0, q1 = _rows("query", query, qs, dt, dev)
+    k, k0, k1 = _rows("key", key, ks, dt, dev)
+    qo, qo0, qo1 = _rows("query_out", q_out, qs, dt, dev)
+    v, v0, v1 = (0, 0, 0) if value is None else _rows("value", value, ks, dt, dev)
+    ko, ko0, ko1 = (0, 0, 0) if k_out is None else _rows("key_out", k_out, ks, dt, dev)
+    if positions.dtype != torch.int32 or positions.shape != (T,) or positions.get_device() != dev \
+            or not positions.is_contiguous():
+        raise _bad(f"positions must be contiguous int32 of shape ({T},) on cuda:{dev}")
+    ts = cos_sin.shape
+    if cos_sin.dtype != torch.float32 or len(ts) != 2 or cos_sin.get_device() != dev or not cos_sin.is_contiguous():
+        raise _bad(f"cos_sin must be contiguous float32 [max_positions, rotary_dim] on cuda:{dev}")
+    code = wcode = dtype_code(dt)
+    qw = kw = 0
+    if q_weight is not None or k_weight is not None:
+        given = [w for w in (q_weight, k_weight) if w is not None]
+        wt = given[0].dtype
+        for w in given:
+            if w.shape != (D,) or w.get_device() != dev or w.dtype != wt or wt not in (dt, torch.float32) \
+                    or not w.is_contiguous():
+                raise _bad(f"norm weights must be contiguous ({D},) on cuda:{dev}, both float32 or both {dt}")
+        wcode = dtype_code(wt)
+        qw = 0 if q_weight is None else q_weight.data_ptr()
+        kw = 0 if k_weight is None else k_weight.data_ptr()
+    try:
+        packed = _ROPE_PARAMS.pack(q, k, v, qo, ko, positions.data_ptr(), cos_sin.data_ptr(), qw, kw, q0, q1, k0, k1,
+                                   v0, v1, qo0, qo1, ko0, ko1, T, H, ks[1], D, ts[1], ts[0], eps,
+                                   1 if interleaved else 0, code, wcode)
+    except struct.error as e:
+        raise _bad(f"a size does not fit 32 bits: {e}") from None
+    return _lib.RopeParams.from_buffer_copy(packed), dev
 
 
 def qk_norm_rope(q_out, k_out, query, key, positions, cos_sin, q_weight=None, k_weight=None, eps=1e-6,
@@ -412,27 +436,29 @@ def qk_norm_rope(q_out, k_out, query, key, positions, cos_sin, q_weight=None, k_
     lib = _lib.load()
     if k_out is None:
         raise _bad("k_out is needed")
-    p = _rope_params(q_out, query, key, positions, cos_sin, q_weight, k_weight, eps, interleaved, k_out=k_out)
-    _on_device(lambda st: lib.cf_qk_norm_rope(ctypes.byref(p), st), query, "cf_qk_norm_rope")
+    p, dev = _rope_params(q_out, query, key, positions, cos_sin, q_weight, k_weight, eps, interleaved, k_out=k_out)
+    _call(lib.cf_qk_norm_rope, dev, "cf_qk_norm_rope", ctypes.byref(p))
 
 
-def _check_caches(key_cache, value_cache, key, dt, slot_mapping):
-    if key_cache.dim() != 4 or key_cache.shape != value_cache.shape or key_cache.shape[1] != key.shape[1] \
-            or key_cache.shape[3] != key.shape[2]:
+def _check_caches(key_cache, value_cache, key, dt, slot_mapping, dev):
+    """Checks the caches and slots of an append; returns (num_blocks, block_size)."""
+    cs, ks = key_cache.shape, key.shape
+    if len(cs) != 4 or value_cache.shape != cs or cs[1] != ks[1] or cs[3] != ks[2]:
         raise _bad("caches must be [num_blocks, num_kv_heads, block_size, head_dim] with key's heads and head_dim")
     for t in (key_cache, value_cache):
-        if t.dtype != dt or not t.is_contiguous() or t.device != key.device:
-            raise _bad(f"caches must be contiguous {dt} on {key.device}")
-    if slot_mapping.dtype != torch.int32 or slot_mapping.shape != (key.shape[0],) \
-            or not slot_mapping.is_contiguous() or slot_mapping.device != key.device:
-        raise _bad(f"slot_mapping must be contiguous int32 of shape ({key.shape[0]},) on {key.device}")
+        if t.dtype != dt or t.get_device() != dev or not t.is_contiguous():
+            raise _bad(f"caches must be contiguous {dt} on cuda:{dev}")
+    if slot_mapping.dtype != torch.int32 or slot_mapping.shape != ks[:1] or slot_mapping.get_device() != dev \
+            or not slot_mapping.is_contiguous():
+        raise _bad(f"slot_mapping must be contiguous int32 of shape ({ks[0]},) on cuda:{dev}")
+    return cs[0], cs[2]
 
 
-def _check_scales(k_scales, v_scales, key_cache):
+def _check_scales(k_scales, v_scales, key_cache, dev):
+    shape = key_cache.shape[:2]
     for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
-        if t.dtype != torch.float32 or t.shape != key_cache.shape[:2] or not t.is_contiguous() \
-                or t.device != key_cache.device:
-            raise _bad(f"{name} must be contiguous float32 {tuple(key_cache.shape[:2])} on {key_cache.device}")
+        if t.dtype != torch.float32 or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+            raise _bad(f"{name} must be contiguous float32 {tuple(shape)} on cuda:{dev}")
 
 
 def rope_and_cache(q_out, query, key, value, key_cache, value_cache, slot_mapping, positions, cos_sin, q_weight=None,
@@ -440,23 +466,20 @@ def rope_and_cache(q_out, query, key, value, key_cache, value_cache, slot_mappin
     """qk_norm_rope with the append in it, one launch: Q goes to q_out, K (normed, rotated) and V to their slots
     of caches of their own dtype, as reshape_and_cache writes them (a negative slot appends nothing)."""
     lib = _lib.load()
-    p = _rope_params(q_out, query, key, positions, cos_sin, q_weight, k_weight, eps, interleaved, value=value)
-    _check_caches(key_cache, value_cache, key, query.dtype, slot_mapping)
-    _on_device(lambda st: lib.cf_rope_and_cache(ctypes.byref(p), _ptr(key_cache), _ptr(value_cache),
-                                                _ptr(slot_mapping), key_cache.shape[2], key_cache.shape[0], st),
-               query, "cf_rope_and_cache")
+    p, dev = _rope_params(q_out, query, key, positions, cos_sin, q_weight, k_weight, eps, interleaved, value)
+    blocks, size = _check_caches(key_cache, value_cache, key, query.dtype, slot_mapping, dev)
+    _call(lib.cf_rope_and_cache, dev, "cf_rope_and_cache", ctypes.byref(p), key_cache.data_ptr(),
+          value_cache.data_ptr(), slot_mapping.data_ptr(), size, blocks)
 
 
 def rope_and_cache_fp8(q_out, query, key, value, key_cache, value_cache, slot_mapping, positions, cos_sin, k_scale,
                        v_scale, q_weight=None, k_weight=None, eps=1e-6, interleaved=False) -> None:
     """rope_and_cache into float8_e4m3fn caches with one scale each: cache = e4m3(x / scale), from the f32 rows."""
     lib = _lib.load()
-    p = _rope_params(q_out, query, key, positions, cos_sin, q_weight, k_weight, eps, interleaved, value=value)
-    _check_caches(key_cache, value_cache, key, torch.float8_e4m3fn, slot_mapping)
-    _on_device(lambda st: lib.cf_rope_and_cache_fp8(ctypes.byref(p), _ptr(key_cache), _ptr(value_cache),
-                                                    _ptr(slot_mapping), key_cache.shape[2], key_cache.shape[0],
-                                                    float(k_scale), float(v_scale), st),
-               query, "cf_rope_and_cache_fp8")
+    p, dev = _rope_params(q_out, query, key, positions, cos_sin, q_weight, k_weight, eps, interleaved, value)
+    blocks, size = _check_caches(key_cache, value_cache, key, torch.float8_e4m3fn, slot_mapping, dev)
+    _call(lib.cf_rope_and_cache_fp8, dev, "cf_rope_and_cache_fp8", ctypes.byref(p), key_cache.data_ptr(),
+          value_cache.data_ptr(), slot_mapping.data_ptr(), size, blocks, float(k_scale), float(v_scale))
 
 
 def rope_and_cache_fp8_block(q_out, query, key, value, key_cache, value_cache, k_scales, v_scales, slot_mapping,
@@ -464,13 +487,11 @@ def rope_and_cache_fp8_block(q_out, query, key, value, key_cache, value_cache, k
     """rope_and_cache into float8_e4m3fn caches with a scale for each block and KV head (rules as
     reshape_and_cache_fp8_block, from the f32 rows)."""
     lib = _lib.load()
-    p = _rope_params(q_out, query, key, positions, cos_sin, q_weight, k_weight, eps, interleaved, value=value)
-    _check_caches(key_cache, value_cache, key, torch.float8_e4m3fn, slot_mapping)
-    _check_scales(k_scales, v_scales, key_cache)
-    _on_device(lambda st: lib.cf_rope_and_cache_fp8_block(ctypes.byref(p), _ptr(key_cache), _ptr(value_cache),
-                                                          _ptr(k_scales), _ptr(v_scales), _ptr(slot_mapping),
-                                                          key_cache.shape[2], key_cache.shape[0], st),
-               query, "cf_rope_and_cache_fp8_block")
+    p, dev = _rope_params(q_out, query, key, positions, cos_sin, q_weight, k_weight, eps, interleaved, value)
+    blocks, size = _check_caches(key_cache, value_cache, key, torch.float8_e4m3fn, slot_mapping, dev)
+    _check_scales(k_scales, v_scales, key_cache, dev)
+    _call(lib.cf_rope_and_cache_fp8_block, dev, "cf_rope_and_cache_fp8_block", ctypes.byref(p), key_cache.data_ptr(),
+          value_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), slot_mapping.data_ptr(), size, blocks)
 
 
 def reshape_and_cache_fp8_block(key, value, key_cache, value_cache, k_scales, v_scales, slot_mapping) -> None:
@@ -484,20 +505,20 @@ def reshape_and_cache_fp8_block(key, value, key_cache, value_cache, k_scales, v_
     block operators take scales.view(num_blocks, num_kv_heads, 1, 1).
     """
     lib = _lib.load()
-    if key.dim() != 3 or key.shape != value.shape or key.dtype != value.dtype or key.device != value.device \
-            or not key.is_cuda:
-        raise _bad("key/value must be CUDA tensors [num_tokens, num_kv_heads, head_dim] of one dtype")
-    T, Hkv, D = key.shape
-    for t in (key, value):
-        if t.stride(2) != 1 and D > 1 or t.stride(1) != D and Hkv > 1:
-            raise _bad("key/value: a token's heads must be contiguous")
-    _check_caches(key_cache, value_cache, key, torch.float8_e4m3fn, slot_mapping)
-    _check_scales(k_scales, v_scales, key_cache)
-    _on_device(lambda st: lib.cf_reshape_and_cache_fp8_block(
-        _ptr(key), _ptr(value), _ptr(key_cache), _ptr(value_cache), _ptr(k_scales), _ptr(v_scales),
-        _ptr(slot_mapping), T, Hkv, D, key.stride(0), value.stride(0), key_cache.shape[2], key_cache.shape[0],
-        dtype_code(key.dtype), st),
-        key, "cf_reshape_and_cache_fp8_block")
+    shape = key.shape
+    if len(shape) != 3 or not key.is_cuda:
+        raise _bad("key/value must be CUDA tensors [num_tokens, num_kv_heads, head_dim]")
+    T, Hkv, D = shape
+    dev = key.get_device()
+    k, k0, k1 = _rows("key", key, shape, key.dtype, dev)
+    v, v0, v1 = _rows("value", value, shape, key.dtype, dev)
+    if (k1 != D or v1 != D) and Hkv > 1:
+        raise _bad("key/value: a token's heads must be contiguous")
+    blocks, size = _check_caches(key_cache, value_cache, key, torch.float8_e4m3fn, slot_mapping, dev)
+    _check_scales(k_scales, v_scales, key_cache, dev)
+    _call(lib.cf_reshape_and_cache_fp8_block, dev, "cf_reshape_and_cache_fp8_block", k, v, key_cache.data_ptr(),
+          value_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), slot_mapping.data_ptr(), T, Hkv, D, k0, v0,
+          size, blocks, dtype_code(key.dtype))
 
 
 def paged_attention_fp8_block_workspace_size(query, key_cache, block_tables, max_context_len) -> int:
@@ -520,25 +541,36 @@ def paged_attention_fp8_block_v1(out, query, key_cache, value_cache, k_scales, v
     head] * stored, V alike; as reshape_and_cache_fp8_block fills them); query and output f16 or bf16, head_dim 128
     or 256.  The workspace (paged_attention_fp8_block_workspace_size bytes) lets long contexts split."""
     lib = _lib.load()
+    qs, cs, bs = query.shape, key_cache.shape, block_tables.shape
+    if len(qs) != 3 or len(cs) != 4 or len(bs) != 2 or out.shape != qs or value_cache.shape != cs or cs[3] != qs[2] \
+            or context_lens.shape != qs[:1] or bs[0] != qs[0] or not query.is_cuda:
+        raise _bad("paged_attention_fp8_block_v1: CUDA tensors; query/out [num_seqs, num_heads, head_dim], caches "
+                   "[num_blocks, num_kv_heads, 16, head_dim], block_tables [num_seqs, max_blocks], context_lens "
+                   "[num_seqs]")
+    dt, dev = query.dtype, query.get_device()
+    for name, t, want in (("query", query, dt), ("out", out, dt), ("key_cache", key_cache, torch.float8_e4m3fn),
+                          ("value_cache", value_cache, torch.float8_e4m3fn), ("block_tables", block_tables, torch.int32),
+                          ("context_lens", context_lens, torch.int32)):
+        if t.dtype != want or t.get_device() != dev or not t.is_contiguous():
+            raise _bad(f"{name} must be contiguous {want} on cuda:{dev}")
+    _check_scales(k_scales, v_scales, key_cache, dev)
     if scale is None:
-        scale = 1.0 / math.sqrt(query.shape[-1])
+        scale = 1.0 / math.sqrt(qs[2])
     if max_context_len is None:
-        max_context_len = int(context_lens.max().item()) if context_lens.numel() else 0
-    p = _attention_params(out, query, key_cache, value_cache, block_tables, context_lens, scale,
-                          max_context_len, fp8=True)
-    S, H, D = query.shape
-    if out.shape != query.shape or value_cache.shape != key_cache.shape or key_cache.shape[3] != D \
-            or context_lens.shape != (S,) or block_tables.dim() != 2 or block_tables.shape[0] != S:
-        raise _bad("paged_attention_fp8_block_v1: shapes of query, out, caches, block_tables and context_lens differ")
-    for t in (out, key_cache, value_cache, block_tables, context_lens):
-        if t.device != query.device:
-            raise _bad(f"paged_attention_fp8_block_v1: every tensor must be on {query.device}")
-    _check_scales(k_scales, v_scales, key_cache)
-    ws = _ptr(workspace)
-    ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
-    _on_device(lambda st: lib.cf_paged_attention_fp8_block_v1(ctypes.byref(p), _ptr(k_scales), _ptr(v_scales), ws,
-                                                              ws_bytes, st),
-               query, "cf_paged_attention_fp8_block_v1")
+        max_context_len = int(context_lens.max().item()) if qs[0] else 0
+    try:
+        packed = _ATTENTION_PARAMS.pack(query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), out.data_ptr(),
+                                        block_tables.data_ptr(), context_lens.data_ptr(), scale, qs[0], qs[1], cs[1],
+                                        qs[2], cs[2], max_context_len, bs[1], cs[0], dtype_code(dt))
+    except struct.error as e:
+        raise _bad(f"a size does not fit 32 bits: {e}") from None
+    p = AttentionParams.from_buffer_copy(packed)
+    ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(),
+                                                        workspace.numel() * workspace.element_size())
+    if workspace is not None and (workspace.get_device() != dev or not workspace.is_contiguous()):
+        raise _bad(f"workspace must be contiguous on cuda:{dev}")
+    _call(lib.cf_paged_attention_fp8_block_v1, dev, "cf_paged_attention_fp8_block_v1", ctypes.byref(p),
+          k_scales.data_ptr(), v_scales.data_ptr(), ws, ws_bytes)
     return out
 
 
