@@ -18,6 +18,7 @@
 // Bound: HBM.  A row is read once and written once; the table row of a token
 // (R floats) is shared by all its heads.
 #include <initializer_list>
+#include <mutex>
 #include <type_traits>
 
 #include "cf_device.cuh"
@@ -561,7 +562,8 @@ struct BlockArgs {
   float* k_scales;  // [num_blocks, Hkv]
   float* v_scales;
   int32_t head_split;  // CTAs per window, each with every head_split-th head
-  int32_t kv_ctas;     // windows * head_split; the CTAs past them take the Q rows
+  int32_t kv_ctas;     // windows * head_split
+  int32_t q_ctas;      // for the Q rows, dealt evenly among the others
 };
 
 struct BlockSmem {
@@ -589,23 +591,31 @@ __device__ __forceinline__ float block_scale(uint32_t bits) {
   return __uint_as_float((uint32_t)e << 23);
 }
 
+constexpr int kTasks = 64;  // (K or V, group of rows, head) copied at once: 64 KB
+constexpr int kStageOffset = (int)((sizeof(BlockSmem) + 127) / 128 * 128);
+// Shared memory of a CTA of either kind.
+template <typename T, int V, int K>
+constexpr int kBlockBytes = K == 1 ? kStageOffset + kTasks * 2 * 32 * V * (int)sizeof(T) : kStageOffset;
+
 template <typename T, int V, int K, bool IL, bool kFull>
-__global__ void __launch_bounds__(kThreads) rope_block_append_kernel(const __grid_constant__ BlockArgs b) {
+__global__ void __launch_bounds__(kThreads, 2) rope_block_append_kernel(const __grid_constant__ BlockArgs b) {
   const RopeArgs& a = b.r;
   constexpr int U = K == 1 ? 2 : 1, kArea = kItemStages * kItemBytes<T, V, K, U>;
-  __shared__ union {
-    BlockSmem sm;
-    __align__(16) uint8_t buffer[kWarps * kArea + 16];
-  } smem;
-  if ((int)blockIdx.x >= b.kv_ctas) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  // Appends wait on memory, Q rows stream it: CTA i is one of the first or of
+  // the second kind so that any stretch of them holds both in proportion.
+  const int64_t ctas = (int64_t)b.kv_ctas + b.q_ctas;
+  const int q_before = (int)((int64_t)blockIdx.x * b.q_ctas / ctas);
+  if ((int64_t)(blockIdx.x + 1) * b.q_ctas / ctas > q_before) {
     const int warp = threadIdx.x >> 5;
-    row_items<T, V, K, U, IL, kFull>(a, (int64_t)(blockIdx.x - b.kv_ctas) * kWarps + warp,
-                                     (int64_t)(gridDim.x - b.kv_ctas) * kWarps, false, smem.buffer + warp * kArea);
+    row_items<T, V, K, U, IL, kFull>(a, (int64_t)q_before * kWarps + warp, (int64_t)b.q_ctas * kWarps, false,
+                                     smem + warp * kArea);
     return;
   }
-  BlockSmem& sm = smem.sm;
+  const int cta = blockIdx.x - q_before;
+  BlockSmem& sm = *reinterpret_cast<BlockSmem*>(smem);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int window = blockIdx.x / b.head_split;
+  const int window = cta / b.head_split;
   const int w0 = window * kBlk;
   const int T_ = a.num_tokens;
 
@@ -691,44 +701,55 @@ __global__ void __launch_bounds__(kThreads) rope_block_append_kernel(const __gri
     if ((lane & 15) == 0) sm.state[l] = (int32_t)((there >> lane) & 0xffffu);
   }
   __syncthreads();
+  if (n == 0) return;  // no row of these blocks is this CTA's
 
-  // 4. the rows, kHeads heads at a time: maxima, scales, bytes.  A warp takes
+  // 4. the rows, some heads at a time: maxima, scales, bytes.  A warp takes
   // 32 / lanes rows of K or V and walks the heads, so the rows' angles and the
   // weights are loaded once; where that leaves warps over, they share the
-  // heads.  The second walk loads and turns the rows again (they are in L1)
-  // unless there was one head to each warp.
+  // heads.  All the vectors of these heads are copied into shared memory at
+  // once (a lane's own slots, 1 KB a warp, row group and head); both walks,
+  // for the maxima and for the bytes, read them there.
   const int sub = lane & ((1 << a.lanes_log2) - 1);
   const int per_warp = 32 >> a.lanes_log2;
   const int groups = (n + per_warp - 1) / per_warp;
   const int sharing = max(1, kWarps / (2 * groups));  // warps per (K or V, group of rows)
+  constexpr int VB = V * (int)sizeof(T);
+  constexpr int kTaskBytes = 2 * 32 * VB;
+  const bool staged = K == 1 && 2 * groups <= kTasks;  // else (rows from all over the call) loaded where used
+  const int at_once = staged ? min(kHeads, kTasks / (2 * groups)) : kHeads;
   Unit un[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) un[k] = unit_of<V, IL, kFull>(a, sub + (k << a.lanes_log2));
+  uint8_t* stage = smem + kStageOffset + lane * VB;
 
-  Raw<T, V> raw[K][2];
   Turn<V> tn[K];
   float f[K][2 * V];
-  auto clear = [&]() {  // what no row or unit fills stays zero
+  auto row = [&](int kv, int e, int head) {  // row e of the list
+    return static_cast<const T*>(kv ? a.v : a.k) + (int64_t)sm.row_tok[e] * (kv ? a.v_ts : a.k_ts) +
+           (int64_t)head * (kv ? a.v_hs : a.k_hs);
+  };
+  auto slot_at = [&](int kv, int group, int hi) { return ((kv * groups + group) * at_once + hi) * kTaskBytes; };
+  auto turns = [&](int kv) { return kv == 0 && (a.k_w != nullptr || a.positions != nullptr); };
+  auto angles = [&](int kv, int e) {
+    if (turns(kv) && e < n)
+      load_turn<T, V, K, IL>(a, a.k_w, a.positions != nullptr ? a.positions[sm.row_tok[e]] : 0, sub, un, tn);
+  };
+  auto values = [&](int kv, int group, int e, int hi, int head) {  // normed and turned, in f
+    Raw<T, V> raw[K][2];
 #pragma unroll
     for (int k = 0; k < K; ++k) raw[k][0] = raw[k][1] = Raw<T, V>{};
-  };
-  auto fetch = [&](int kv, int e, int head) {  // row e of the list
-    if (e < n) {
-      const T* p = static_cast<const T*>(kv ? a.v : a.k) + (int64_t)sm.row_tok[e] * (kv ? a.v_ts : a.k_ts) +
-                   (int64_t)head * (kv ? a.v_hs : a.k_hs);
+    if (K == 1 && staged) {
+      const uint8_t* p = stage + slot_at(kv, group, hi);
+      raw[0][0] = *reinterpret_cast<const Raw<T, V>*>(p);
+      raw[0][1] = *reinterpret_cast<const Raw<T, V>*>(p + 32 * VB);
+    } else if (e < n) {
+      const T* p = row(kv, e, head);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         if (un[k].has1) raw[k][0] = *reinterpret_cast<const Raw<T, V>*>(p + un[k].o1);
         if (un[k].has2) raw[k][1] = *reinterpret_cast<const Raw<T, V>*>(p + un[k].o2);
       }
     }
-  };
-  auto turns = [&](int kv) { return kv == 0 && (a.k_w != nullptr || a.positions != nullptr); };
-  auto angles = [&](int kv, int e) {
-    if (turns(kv) && e < n)
-      load_turn<T, V, K, IL>(a, a.k_w, a.positions != nullptr ? a.positions[sm.row_tok[e]] : 0, sub, un, tn);
-  };
-  auto values = [&](int kv) {  // what was fetched, normed and turned
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       unpack<T, V>(raw[k][0], f[k]);
@@ -736,12 +757,36 @@ __global__ void __launch_bounds__(kThreads) rope_block_append_kernel(const __gri
     }
     if (turns(kv)) norm_turn<V, K, IL>(a, f, a.k_w != nullptr, un, tn);
   };
-  const int mine = blockIdx.x % b.head_split;  // heads mine, mine + head_split, ...
+  const int mine = cta % b.head_split;  // heads mine, mine + head_split, ...
   const int heads = (a.num_kv_heads - mine + b.head_split - 1) / b.head_split;
-  for (int h0 = 0; h0 < heads; h0 += kHeads) {
-    const int nh = min(kHeads, heads - h0);
+#pragma unroll 1
+  for (int h0 = 0; h0 < heads; h0 += at_once) {
+    const int nh = min(at_once, heads - h0);
     auto head_of = [&](int i) { return mine + (h0 + i) * b.head_split; };
+    // (K or V, group of rows, share of the heads) of this warp
+    auto walk = [&](auto&& work) {
+#pragma unroll 1
+      for (int c = warp; c < 2 * groups * sharing; c += kWarps) {
+        const int kv = c % 2, group = c / 2 % groups;
+        work(kv, group, group * per_warp + (lane >> a.lanes_log2), c / (2 * groups));
+      }
+    };
     if (h0 > 0) __syncthreads();
+    if constexpr (K == 1) {
+      if (staged)
+        walk([&](int kv, int group, int e, int share) {
+          const bool there = e < n;
+          const uint32_t dst = smem_addr(stage) + slot_at(kv, group, 0);
+          const T* p = there ? row(kv, e, head_of(share)) : static_cast<const T*>(a.k);
+          const int64_t step = there ? (int64_t)(kv ? a.v_hs : a.k_hs) * sharing * b.head_split : 0;
+          for (int hi = share; hi < nh; hi += sharing, p += step) {
+            copy_or_zero<VB>(dst + hi * kTaskBytes, p + (there && un[0].has1 ? un[0].o1 : 0), there && un[0].has1);
+            copy_or_zero<VB>(dst + hi * kTaskBytes + 32 * VB, p + (there && un[0].has2 ? un[0].o2 : 0),
+                             there && un[0].has2);
+          }
+        });
+      cp_async_commit();
+    }
     for (int i = tid; i < 2 * kHeads * kBlk; i += kThreads) {
       const int kv = i / (kHeads * kBlk), hi = i / kBlk % kHeads, l = i % kBlk;
       float s = 0.f;
@@ -751,28 +796,25 @@ __global__ void __launch_bounds__(kThreads) rope_block_append_kernel(const __gri
       sm.top[kv][hi][l] = 0u;
     }
     __syncthreads();
-    const bool once = 2 * groups * sharing <= kWarps && nh <= sharing;
-    auto walk = [&](auto&& work) {
-      for (int c = warp; c < 2 * groups * sharing; c += kWarps) {
-        const int kv = c % 2, e = c / 2 % groups * per_warp + (lane >> a.lanes_log2);
-        work(kv, e, c / (2 * groups));
-      }
-    };
-    walk([&](int kv, int e, int share) {
-      clear();
+    const bool once = 2 * groups * sharing <= kWarps;  // a warp has one kind and group: its angles stay
+    walk([&](int kv, int group, int e, int share) {
       angles(kv, e);
-      if (share < nh) fetch(kv, e, head_of(share));
+      if (K == 1) cp_async_wait_all();
+#pragma unroll 1
       for (int hi = share; hi < nh; hi += sharing) {
-        values(kv);
-        if (hi + sharing < nh) fetch(kv, e, head_of(hi + sharing));
-        float top = 0.f;
+        values(kv, group, e, hi, head_of(hi));
+        float top = 0.f;  // over the finite values: fmaxf leaves NaN out, infinities are looked for after
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-          for (int i = 0; i < 2 * V; ++i) {
-            const float x = fabsf(f[k][i]);
-            top = fmaxf(top, x <= 3.402823466e38f ? x : 0.f);
-          }
+          for (int i = 0; i < 2 * V; ++i) top = fmaxf(top, fabsf(f[k][i]));
+        if (top == INFINITY) {
+          top = 0.f;
+#pragma unroll
+          for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < 2 * V; ++i) top = fmaxf(top, fabsf(f[k][i]) == INFINITY ? 0.f : fabsf(f[k][i]));
+        }
         for (int m = (1 << a.lanes_log2) >> 1; m > 0; m >>= 1) top = fmaxf(top, shfl_xor(top, m));
         if (e < n && sub == 0) atomicMax(&sm.top[kv][hi][sm.row_lo[e] / kBlk], __float_as_uint(top));
       }
@@ -787,30 +829,25 @@ __global__ void __launch_bounds__(kThreads) rope_block_append_kernel(const __gri
       (kv ? b.v_scales : b.k_scales)[(int64_t)sm.lead[l] * a.num_kv_heads + head_of(hi)] = s;
     }
     __syncthreads();
-    walk([&](int kv, int e, int share) {
+    walk([&](int kv, int group, int e, int share) {
       uint8_t* cache = static_cast<uint8_t*>(kv ? a.vc : a.kc);
       const int l = e < n ? sm.row_lo[e] / kBlk : 0, off = e < n ? sm.row_lo[e] % kBlk : 0;
       const int64_t block = (int64_t)sm.lead[l] * a.num_kv_heads;
-      if (!once) {
-        clear();
-        angles(kv, e);
-        if (share < nh) fetch(kv, e, head_of(share));
-      }
+      if (!once) angles(kv, e);
+#pragma unroll 1
       for (int hi = share; hi < nh; hi += sharing) {
-        if (!once) {
-          values(kv);
-          if (hi + sharing < nh) fetch(kv, e, head_of(hi + sharing));
-        }
+        if (!(once && nh <= sharing)) values(kv, group, e, hi, head_of(hi));  // one head: still in f
         if (e >= n) continue;
         const float s = sm.now[kv][hi][l];
         uint8_t* dst = cache + ((block + head_of(hi)) * kBlk + off) * a.head_dim;
         const uint32_t bits = __float_as_uint(s);
         if ((bits & 0x7fffffu) == 0u && bits >= (1u << 23) && bits < (254u << 23)) {
           const float inv = __uint_as_float((254u << 23) - bits);  // x / 2^k = x 2^-k, exactly
+          const Pair r = pair(inv, inv);
 #pragma unroll
           for (int k = 0; k < K; ++k)
 #pragma unroll
-            for (int i = 0; i < 2 * V; ++i) f[k][i] *= inv;
+            for (int i = 0; i < 2 * V; i += 2) split(mul2(pair(f[k][i], f[k][i + 1]), r), f[k][i], f[k][i + 1]);
         } else if (s > 0.f) {  // a pool may hold scales that are no powers of two
 #pragma unroll
           for (int k = 0; k < K; ++k)
@@ -949,31 +986,48 @@ cf_status launch_rows_type(RopeArgs& a, bool interleaved, cudaStream_t stream) {
   return launch_rows<T, 1, 4>(a, interleaved, stream);
 }
 
+// Per kernel instantiation and device: opt in to > 48 KB of dynamic smem.
+template <typename T, int V, int K, bool IL, bool kFull>
+cf_status launch_block_kernel(const BlockArgs& b, unsigned grid, cudaStream_t stream) {
+  static std::once_flag flags[64];
+  static cudaError_t errs[64];
+  auto kern = rope_block_append_kernel<T, V, K, IL, kFull>;
+  constexpr int bytes = kBlockBytes<T, V, K>;
+  auto set = [&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); };
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) {
+    if (dev >= 0 && dev < 64) {
+      std::call_once(flags[dev], [&] { errs[dev] = set(); });
+      e = errs[dev];
+    } else {
+      e = set();
+    }
+  }
+  if (e != cudaSuccess) return cuda_status(e);
+  kern<<<grid, kThreads, bytes, stream>>>(b);
+  return check_launch();
+}
+
 template <typename T, int V, int K>
 cf_status launch_block(BlockArgs b, bool interleaved, cudaStream_t stream) {
   const RopeArgs& a = b.r;
   const int windows = (a.num_tokens + kBlk - 1) / kBlk;
-  // about four CTAs per SM: a CTA per (window, head) for decode steps, whole
-  // windows once there are enough of them
-  const int target = 4 * sm_count();
+  // about two CTAs per SM, as many as are resident: a CTA per (window, head)
+  // for decode steps, whole windows once there are enough of them
+  const int target = 2 * sm_count();
   int split = (target + windows - 1) / windows;
   b.head_split = split < 1 ? 1 : (split > a.num_kv_heads ? a.num_kv_heads : split);
   b.kv_ctas = windows * b.head_split;
-  const unsigned grid = b.kv_ctas + (a.num_heads > 0 ? row_ctas(a, K == 1 ? 2 : 1, kWarps, {a.num_heads}) : 0);
+  b.q_ctas = a.num_heads > 0 ? (int32_t)row_ctas(a, K == 1 ? 2 : 1, kWarps, {a.num_heads}) : 0;
+  const unsigned grid = (unsigned)(b.kv_ctas + b.q_ctas);
   if constexpr (K == 1) {
-    if (full_rows(a)) {
-      if (interleaved)
-        rope_block_append_kernel<T, V, K, true, true><<<grid, kThreads, 0, stream>>>(b);
-      else
-        rope_block_append_kernel<T, V, K, false, true><<<grid, kThreads, 0, stream>>>(b);
-      return check_launch();
-    }
+    if (full_rows(a))
+      return interleaved ? launch_block_kernel<T, V, K, true, true>(b, grid, stream)
+                         : launch_block_kernel<T, V, K, false, true>(b, grid, stream);
   }
-  if (interleaved)
-    rope_block_append_kernel<T, V, K, true, false><<<grid, kThreads, 0, stream>>>(b);
-  else
-    rope_block_append_kernel<T, V, K, false, false><<<grid, kThreads, 0, stream>>>(b);
-  return check_launch();
+  return interleaved ? launch_block_kernel<T, V, K, true, false>(b, grid, stream)
+                     : launch_block_kernel<T, V, K, false, false>(b, grid, stream);
 }
 
 template <typename T>
