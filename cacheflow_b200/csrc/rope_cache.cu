@@ -351,9 +351,8 @@ __device__ __forceinline__ void copy_or_zero(uint32_t dst, const void* src, bool
                : "memory");
 }
 
-template <typename T, int V, int K, int U, bool IL, bool kFull>
-__device__ __forceinline__ void row_items(const RopeArgs& a, int64_t warp, int64_t num_warps, bool with_kv,
-                                          uint8_t* buffer) {
+template <typename T, int V, int K, int U, bool IL, bool kFull, bool kKv>
+__device__ __forceinline__ void row_items(const RopeArgs& a, int64_t warp, int64_t num_warps, uint8_t* buffer) {
   constexpr bool kPipe = K == 1;  // (a lane of one-element vectors loads where it uses them)
   constexpr int VB = V * (int)sizeof(T);
   const int lane = threadIdx.x & 31;
@@ -361,7 +360,7 @@ __device__ __forceinline__ void row_items(const RopeArgs& a, int64_t warp, int64
   const int per_warp = 32 >> a.lanes_log2;
   const int grp = lane >> a.lanes_log2;
   const int nq = (a.num_heads + per_warp * U - 1) / (per_warp * U);
-  const int nk = with_kv ? (a.num_kv_heads + per_warp * U - 1) / (per_warp * U) : 0;
+  const int nk = kKv ? (a.num_kv_heads + per_warp * U - 1) / (per_warp * U) : 0;
   const int per_token = nq + nk + (a.dest == kDense ? 0 : nk);
   Unit un[K];
 #pragma unroll
@@ -388,7 +387,7 @@ __device__ __forceinline__ void row_items(const RopeArgs& a, int64_t warp, int64
     look(x);
     return x;
   };
-  auto kind_of = [&](int c) { return c < nq ? 0 : (c < nq + nk ? 1 : 2); };
+  auto kind_of = [&](int c) { return !kKv || c < nq ? 0 : (c < nq + nk ? 1 : 2); };
   auto heads_of = [&](int kind) { return kind == 0 ? a.num_heads : a.num_kv_heads; };
   auto head_of = [&](int c, int kind) { return (kind == 0 ? c : kind == 1 ? c - nq : c - nq - nk) * per_warp * U + grp; };
   auto stride_of = [&](int kind) { return kind == 0 ? a.q_hs : kind == 1 ? a.k_hs : a.v_hs; };
@@ -505,7 +504,7 @@ __device__ __forceinline__ void row_items(const RopeArgs& a, int64_t warp, int64
     using Y = std::true_type;
     using N = std::false_type;
     const bool fp8 = cached && a.dest == kCacheFp8;
-    if (kind < 2 && !fp8)
+    if (!kKv || (kind < 2 && !fp8))
       head0 - grp + U * per_warp <= heads ? finish(Y{}, N{}, Y{}) : finish(Y{}, N{}, N{});
     else if (kind < 2)
       finish(Y{}, Y{}, N{});
@@ -525,8 +524,8 @@ __global__ void __launch_bounds__(kRowThreads) rope_rows_kernel(const __grid_con
   constexpr int kArea = kItemStages * kItemBytes<T, V, K, U>;
   __shared__ __align__(16) uint8_t buffer[kRowWarps * kArea + 16];
   const int warp = threadIdx.x >> 5;
-  row_items<T, V, K, U, IL, kFull>(a, (int64_t)blockIdx.x * kRowWarps + warp, (int64_t)gridDim.x * kRowWarps, true,
-                                   buffer + warp * kArea);
+  row_items<T, V, K, U, IL, kFull, true>(a, (int64_t)blockIdx.x * kRowWarps + warp, (int64_t)gridDim.x * kRowWarps,
+                                         buffer + warp * kArea);
 }
 
 // ---------------------------------------------------------------------------
@@ -608,8 +607,8 @@ __global__ void __launch_bounds__(kThreads, 2) rope_block_append_kernel(const __
   const int q_before = (int)((int64_t)blockIdx.x * b.q_ctas / ctas);
   if ((int64_t)(blockIdx.x + 1) * b.q_ctas / ctas > q_before) {
     const int warp = threadIdx.x >> 5;
-    row_items<T, V, K, U, IL, kFull>(a, (int64_t)q_before * kWarps + warp, (int64_t)b.q_ctas * kWarps, false,
-                                     smem + warp * kArea);
+    row_items<T, V, K, U, IL, kFull, false>(a, (int64_t)q_before * kWarps + warp, (int64_t)b.q_ctas * kWarps,
+                                            smem + warp * kArea);
     return;
   }
   const int cta = blockIdx.x - q_before;
@@ -640,36 +639,59 @@ __global__ void __launch_bounds__(kThreads, 2) rope_block_append_kernel(const __
   __syncthreads();
   bool leads = false;
   if (tid < kBlk) {
-    leads = key >= 0;
-    for (int j = 0; j < tid; ++j) leads = leads && sm.key[j] != key;
+    int first = tid;  // of the window's tokens in this block
+    for (int j = kBlk - 1; j >= 0; --j)
+      if (j < first && sm.key[j] == key) first = j;
+    leads = key >= 0 && first == tid;
     sm.lead[tid] = leads ? key : -1;
     if (leads) atomicOr(&sm.filter[(key >> 5) & 31], 1u << (key & 31));
+    if (key >= 0) atomicMax(&sm.win[first][a.slots[w0 + tid] % kBlk], w0 + tid);
   }
   if (__syncthreads_or(leads ? 1 : 0) == 0) return;  // padding only
 
-  // 2. their tokens, wherever they are in the call (16 loads in flight)
-  constexpr int kLook = 16;
-  for (int i0 = tid; i0 < T_; i0 += kThreads * kLook) {
-    int slot[kLook];
-#pragma unroll
-    for (int u = 0; u < kLook; ++u) {
-      const int i = i0 + u * kThreads;
-      slot[u] = i < T_ ? a.slots[i] : -1;
+  // 2. their tokens outside the window, wherever they are in the call (seldom
+  // more than a run that goes on behind it): four slots a load where they are
+  // 16-byte aligned, eight loads in flight (16384 slots one at a time and 16 in
+  // flight took 5.3 us of a CTA's 17)
+  auto hit = [&](int slot) -> uint32_t {
+    const int k = slot / kBlk;
+    return slot >= 0 ? (sm.filter[(k >> 5) & 31] >> (k & 31)) & 1u : 0u;
+  };
+  auto match = [&](int i) {
+    const int slot = a.slots[i], k = slot / kBlk;
+#pragma unroll 1
+    for (int l = 0; l < kBlk; ++l) {
+      if (sm.lead[l] != k) continue;
+      if (i < w0)
+        sm.dead[l] = 1;
+      else
+        atomicMax(&sm.win[l][slot % kBlk], i);
     }
+  };
+  constexpr int kLook = 8;
+  const int quads = (reinterpret_cast<uintptr_t>(a.slots) & 15) == 0 ? T_ / 4 : 0;
+#pragma unroll 1
+  for (int q0 = tid; q0 < quads; q0 += kThreads * kLook) {
+    int4 slot[kLook];
 #pragma unroll
     for (int u = 0; u < kLook; ++u) {
-      if (slot[u] < 0) continue;
-      const int k = slot[u] / kBlk, i = i0 + u * kThreads;
-      if (!((sm.filter[(k >> 5) & 31] >> (k & 31)) & 1u)) continue;
-      for (int l = 0; l < kBlk; ++l) {
-        if (sm.lead[l] != k) continue;
-        if (i < w0)
-          sm.dead[l] = 1;
-        else
-          atomicMax(&sm.win[l][slot[u] % kBlk], i);
-      }
+      const int q = q0 + u * kThreads;
+      const bool look = q < quads && (uint32_t)(q - w0 / 4) >= (uint32_t)(kBlk / 4);
+      slot[u] = look ? reinterpret_cast<const int4*>(a.slots)[q] : make_int4(-1, -1, -1, -1);
+    }
+    uint32_t hits = 0u;
+#pragma unroll
+    for (int u = 0; u < kLook; ++u)
+      hits |= (hit(slot[u].x) | hit(slot[u].y) << 1 | hit(slot[u].z) << 2 | hit(slot[u].w) << 3) << (4 * u);
+#pragma unroll 1
+    for (; hits != 0u; hits &= hits - 1u) {
+      const int j = __ffs(hits) - 1;
+      match((q0 + j / 4 * kThreads) * 4 + j % 4);
     }
   }
+#pragma unroll 1
+  for (int i = 4 * quads + tid; i < T_; i += kThreads)
+    if ((uint32_t)(i - w0) >= (uint32_t)kBlk && hit(a.slots[i])) match(i);
   __syncthreads();
 
   // 3. the rows to append, in (block, offset) order
