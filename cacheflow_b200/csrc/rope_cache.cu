@@ -17,6 +17,7 @@
 //
 // Bound: HBM.  A row is read once and written once; the table row of a token
 // (R floats) is shared by all its heads.
+#include <atomic>
 #include <initializer_list>
 #include <mutex>
 #include <type_traits>
@@ -599,7 +600,7 @@ constexpr int kBlockBytes = K == 1 ? kStageOffset + kTasks * 2 * 32 * V * (int)s
 template <typename T, int V, int K, bool IL, bool kFull>
 __global__ void __launch_bounds__(kThreads, 2) rope_block_append_kernel(const __grid_constant__ BlockArgs b) {
   const RopeArgs& a = b.r;
-  constexpr int U = K == 1 ? 2 : 1, kArea = kItemStages * kItemBytes<T, V, K, U>;
+  constexpr int U = K == 1 ? 4 : 1, kArea = kItemStages * kItemBytes<T, V, K, U>;
   extern __shared__ __align__(16) uint8_t smem[];
   // Appends wait on memory, Q rows stream it: CTA i is one of the first or of
   // the second kind so that any stretch of them holds both in proportion.
@@ -952,50 +953,64 @@ int row_layout(RopeArgs& a, int v) {
 // Whether every lane of a row has a unit that rotates.
 bool full_rows(const RopeArgs& a) { return a.rotary == a.head_dim && a.units == (1 << a.lanes_log2); }
 
-// CTAs of `warps` warps for the row items of `heads` (a count per kind, 0 for none).
-unsigned row_ctas(const RopeArgs& a, int u, int warps, std::initializer_list<int> heads) {
+// CTAs of `warps` warps for the row items of `heads` (a count per kind, 0 for
+// none), at most `cap`.
+unsigned row_ctas(const RopeArgs& a, int u, int warps, int64_t cap, std::initializer_list<int> heads) {
   const int rows = (32 >> a.lanes_log2) * u;
   int64_t items = 0;
   for (int h : heads) items += (h + rows - 1) / rows;
   items *= a.num_tokens;
-  const int64_t want = (items + warps - 1) / warps, cap = (int64_t)sm_count() * 64 / warps;
+  const int64_t want = (items + warps - 1) / warps;
   return (unsigned)(want < cap ? want : cap);
 }
 
-template <typename T, int V, int K, int U>
-cf_status launch_rows_u(const RopeArgs& a, bool interleaved, unsigned grid, cudaStream_t stream) {
-  if constexpr (K == 1) {
-    if (full_rows(a)) {
-      if (interleaved)
-        rope_rows_kernel<T, V, K, U, true, true><<<grid, kRowThreads, 0, stream>>>(a);
-      else
-        rope_rows_kernel<T, V, K, U, false, true><<<grid, kRowThreads, 0, stream>>>(a);
-      return check_launch();
-    }
+// Runs as many CTAs as are resident at once: each walks its items with the
+// next one's copies in flight (8192 tokens of 64 / 8 heads 60 us, 76 with a
+// quarter more CTAs than that, 63 with four times as many).
+template <typename T, int V, int K, int U, bool IL, bool kFull>
+cf_status launch_rows_kernel(const RopeArgs& a, cudaStream_t stream) {
+  static std::atomic<int> resident[64];
+  auto kern = rope_rows_kernel<T, V, K, U, IL, kFull>;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_status(e);
+  int per_sm = dev < 64 ? resident[dev].load(std::memory_order_relaxed) : 0;
+  if (per_sm == 0) {
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kRowThreads, 0);
+    if (e != cudaSuccess) return cuda_status(e);
+    per_sm = per_sm < 1 ? 1 : per_sm;
+    if (dev < 64) resident[dev].store(per_sm, std::memory_order_relaxed);
   }
-  if (interleaved)
-    rope_rows_kernel<T, V, K, U, true, false><<<grid, kRowThreads, 0, stream>>>(a);
-  else
-    rope_rows_kernel<T, V, K, U, false, false><<<grid, kRowThreads, 0, stream>>>(a);
+  const unsigned grid = row_ctas(a, U, kRowWarps, (int64_t)sm_count() * per_sm,
+                                 {a.num_heads, a.num_kv_heads, a.dest == kDense ? 0 : a.num_kv_heads});
+  kern<<<grid, kRowThreads, 0, stream>>>(a);
   return check_launch();
+}
+
+template <typename T, int V, int K, int U>
+cf_status launch_rows_u(const RopeArgs& a, bool interleaved, cudaStream_t stream) {
+  if constexpr (K == 1) {
+    if (full_rows(a))
+      return interleaved ? launch_rows_kernel<T, V, K, U, true, true>(a, stream)
+                         : launch_rows_kernel<T, V, K, U, false, true>(a, stream);
+  }
+  return interleaved ? launch_rows_kernel<T, V, K, U, true, false>(a, stream)
+                     : launch_rows_kernel<T, V, K, U, false, false>(a, stream);
 }
 
 template <typename T, int V, int K>
 cf_status launch_rows(const RopeArgs& a, bool interleaved, cudaStream_t stream) {
-  auto ctas = [&](int u) {
-    return row_ctas(a, u, kRowWarps, {a.num_heads, a.num_kv_heads, a.dest == kDense ? 0 : a.num_kv_heads});
-  };
   if constexpr (K == 1) {
     // Heads per lane group and item: four 16-bit rows (8192 tokens of 64 / 8
     // heads 64 us, 77 with two), two f32 ones (4095 tokens of 32 / 32 heads 29
     // us, 32 with four), one where a call has few items (a token of 32 / 8
-    // heads 3.8 us, 4.3 with four).
+    // heads 3.7 us, 4.3 with four).
     constexpr int U = sizeof(T) == 4 ? 2 : 4;
-    const unsigned grid = ctas(U);
-    if (grid < (unsigned)sm_count()) return launch_rows_u<T, V, K, 1>(a, interleaved, ctas(1), stream);
-    return launch_rows_u<T, V, K, U>(a, interleaved, grid, stream);
+    const unsigned ctas = row_ctas(a, U, kRowWarps, INT32_MAX, {a.num_heads, a.num_kv_heads, a.num_kv_heads});
+    return ctas < (unsigned)sm_count() ? launch_rows_u<T, V, K, 1>(a, interleaved, stream)
+                                       : launch_rows_u<T, V, K, U>(a, interleaved, stream);
   }
-  return launch_rows_u<T, V, K, 1>(a, interleaved, ctas(1), stream);
+  return launch_rows_u<T, V, K, 1>(a, interleaved, stream);
 }
 
 template <typename T>
@@ -1041,7 +1056,9 @@ cf_status launch_block(BlockArgs b, bool interleaved, cudaStream_t stream) {
   int split = (target + windows - 1) / windows;
   b.head_split = split < 1 ? 1 : (split > a.num_kv_heads ? a.num_kv_heads : split);
   b.kv_ctas = windows * b.head_split;
-  b.q_ctas = a.num_heads > 0 ? (int32_t)row_ctas(a, K == 1 ? 2 : 1, kWarps, {a.num_heads}) : 0;
+  // (16384 tokens of 32 / 8 heads 126 us with at most four Q CTAs per SM, 131
+  // with eight, 152 with two)
+  b.q_ctas = a.num_heads > 0 ? (int32_t)row_ctas(a, K == 1 ? 4 : 1, kWarps, 4 * sm_count(), {a.num_heads}) : 0;
   const unsigned grid = (unsigned)(b.kv_ctas + b.q_ctas);
   if constexpr (K == 1) {
     if (full_rows(a))
