@@ -23,11 +23,23 @@ its output only after it was copied out.
 
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
 
-from . import ops
+from . import _lib, ops
 
 V1_MAX_CONTEXT = 8192  # batch_decode.cpp:163
+
+
+class Rotation(NamedTuple):
+    """Norms and rotation that an engine applies to queries and new keys before they are used (ops.qk_norm_rope)."""
+
+    cos_sin: torch.Tensor
+    q_weight: torch.Tensor | None = None
+    k_weight: torch.Tensor | None = None
+    eps: float = 1e-6
+    interleaved: bool = False
 
 
 class _Slot:
@@ -37,6 +49,7 @@ class _Slot:
         self.k_new = torch.empty((max_new, num_kv_heads, head_dim), dtype=dt, device=dev)
         self.v_new = torch.empty_like(self.k_new)
         self.slots = torch.empty((max_new,), dtype=torch.int32, device=dev)
+        self.pos = torch.empty((max_new,), dtype=torch.int32, device=dev)
         self.tables = torch.empty((max_seqs, max_blocks), dtype=torch.int32, device=dev)
         self.ctx = torch.empty((max_seqs,), dtype=torch.int32, device=dev)
         self.c_tables = torch.empty((max_chunks, max_blocks), dtype=torch.int32, device=dev)
@@ -53,14 +66,24 @@ class DecodeEngine:
                  max_seqs: int, max_blocks_per_seq: int, max_new_tokens: int | None = None,
                  stream: torch.cuda.Stream | None = None, split_v1: bool = True, depth: int = 2,
                  max_chunks: int = 0, fused_append: bool = False, kv_scales: tuple[float, float] | None = None,
-                 query_dtype: torch.dtype | None = None, kernel: str = "v1"):
+                 query_dtype: torch.dtype | None = None, kernel: str = "v1", rotation: Rotation | None = None):
         """kv_scales = (k_scale, v_scale) with float8_e4m3fn caches: the caches
         hold K / k_scale and V / v_scale; queries, new K/V rows and outputs are
-        `query_dtype` (f16 / bf16).  kernel = "v1" (v1 with the library's
+        `query_dtype` (f16 / bf16).  Two float32 tensors [num_blocks,
+        num_kv_heads] instead are scales for each block and KV head, kept by
+        the appends (ops.reshape_and_cache_fp8_block).  kernel = "v1" (v1 with the library's
         split at every context length) or "reference" (v1 up to 8192 tokens,
-        v2 beyond, as CacheFlow's engine chooses)."""
+        v2 beyond, as CacheFlow's engine chooses).  With a rotation, step()
+        and attend() take queries and keys as the projection gives them, one
+        new token for each query row and its position."""
         if kernel not in ("v1", "reference"):
             raise ValueError("kernel must be 'v1' or 'reference'")
+        self.rotation = rotation
+        self.block_scaled = kv_scales is not None and isinstance(kv_scales[0], torch.Tensor)
+        if self.block_scaled and (kernel != "v1" or fused_append or key_cache.dtype != torch.float8_e4m3fn):
+            raise ValueError("block scales: float8_e4m3fn caches, kernel='v1', fused_append=False")
+        if rotation is not None and fused_append:
+            raise ValueError("a rotation appends in its own launch: fused_append=False")
         self.k = key_cache
         self.v = value_cache
         self.device = key_cache.device
@@ -90,7 +113,9 @@ class DecodeEngine:
         self.workspace = None
         if split_v1:
             v1_ctx = max_ctx if self.v2_above is None else min(max_ctx, self.v2_above)
-            n = ops.paged_attention_v1_workspace_size(self.q, key_cache, self.tables, v1_ctx)
+            size = (ops.paged_attention_fp8_block_workspace_size if self.block_scaled
+                    else ops.paged_attention_v1_workspace_size)
+            n = size(self.q, key_cache, self.tables, v1_ctx)
             if n:
                 self.workspace = torch.empty((n,), dtype=torch.uint8, device=dev)
         self.parts = ops.v2_num_partitions(max_ctx)
@@ -109,7 +134,8 @@ class DecodeEngine:
     def h2d_bytes(self, num_seqs: int, num_new: int) -> int:
         e = self.q.element_size()
         return (num_seqs * self.num_heads * self.head_dim * e + 2 * num_new * self.num_kv_heads * self.head_dim * e
-                + num_new * 4 + num_seqs * self.max_blocks_per_seq * 4 + num_seqs * 4)
+                + num_new * (4 if self.rotation is None else 8) + num_seqs * self.max_blocks_per_seq * 4
+                + num_seqs * 4)
 
     def d2h_bytes(self, num_seqs: int) -> int:
         return num_seqs * self.num_heads * self.head_dim * self.q.element_size()
@@ -117,10 +143,31 @@ class DecodeEngine:
     def _use_v2(self, max_context_len: int) -> bool:
         return self.v2_above is not None and max_context_len > self.v2_above
 
+    def _rotate_append(self, q, k_new, v_new, slots, positions) -> None:
+        """Queries normed and rotated in place, new keys normed, rotated and appended with their values."""
+        r = self.rotation
+        rows = (q, q, k_new, v_new, self.k, self.v)
+        norms = {"q_weight": r.q_weight, "k_weight": r.k_weight, "eps": r.eps, "interleaved": r.interleaved}
+        if self.block_scaled:
+            ops.rope_and_cache_fp8_block(*rows, *self.kv_scales, slots, positions, r.cos_sin, **norms)
+        elif self.fp8:
+            ops.rope_and_cache_fp8(*rows, slots, positions, r.cos_sin, *self.kv_scales, **norms)
+        else:
+            ops.rope_and_cache(*rows, slots, positions, r.cos_sin, **norms)
+
     def _attend(self, q, out, bt, cl, num_seqs: int, max_context_len: int, new=None) -> None:
         """new = (k_new, v_new, slot_mapping) of one token per row appends it
         in the same launch."""
         S = num_seqs
+        if self.block_scaled:
+            if new is not None:
+                ops.reshape_and_cache_fp8_block(new[0], new[1], self.k, self.v, *self.kv_scales, new[2])
+            ops.paged_attention_fp8_block_v1(out, q, self.k, self.v, *self.kv_scales, bt, cl, None, max_context_len,
+                                             workspace=self.workspace)
+            split = self.workspace is not None and ops.paged_attention_fp8_block_workspace_size(
+                q, self.k, bt, max_context_len) > 0
+            self.launches_per_step = (2 if split else 1) + (1 if new is not None else 0)
+            return
         if self.fp8:
             ks, vs = self.kv_scales
             fused = new is not None and self.fused_append
@@ -174,6 +221,8 @@ class DecodeEngine:
         decode rows (HBM-bound) on a high-priority side stream forked from it
         and joined back into it, so the decode CTAs take SMs as the prefill's
         retire instead of waiting for the whole prefill grid."""
+        if self.fp8:
+            raise ops.CacheFlowError(_lib.CF_ERR_UNSUPPORTED, "prefill chunks attend over 16-bit caches")
         nd, nc, max_q = chunks
         cur = torch.cuda.current_stream(self.device)
         if nd:
@@ -191,21 +240,30 @@ class DecodeEngine:
             cur.wait_event(self.joined)
         self.launches_per_step += 1
 
-    def attend(self, num_seqs: int, max_context_len: int, chunks=None, new=None) -> None:
+    def attend(self, num_seqs: int, max_context_len: int, chunks=None, new=None, positions=None) -> None:
         """Attention over inputs already in self.q / self.tables / self.ctx
         (the device-resident path), output in self.out; current stream.
         chunks = (num_decode, num_chunks, max_chunk_len) runs rows past
         num_decode as prefill chunks (self.c_tables / c_ctx / c_start).
         new = (k_new, v_new, slot_mapping), one token per row at its newest
-        position, is appended to the cache in the same launch."""
+        position, is appended to the cache in the same launch.  An engine with
+        a rotation appends before it attends: new and positions (int32
+        [num_seqs]) are of every query row, and self.q is rotated in place."""
         S = num_seqs
+        extra = 0
+        if self.rotation is not None:
+            if new is None or positions is None:
+                raise ValueError("a rotation needs the new tokens and their positions")
+            self._rotate_append(self.q[:S], *new, positions)
+            new, extra = None, 1
         if chunks is not None:
             self._attend_mixed(self.slots_[0], S, max_context_len, chunks)
-            return
-        self._attend(self.q[:S], self.out[:S], self.tables[:S], self.ctx[:S], S, max_context_len, new)
+        else:
+            self._attend(self.q[:S], self.out[:S], self.tables[:S], self.ctx[:S], S, max_context_len, new)
+        self.launches_per_step += extra
 
     def step(self, q_host, k_new_host, v_new_host, slots_host, tables_host, ctx_host, out_host,
-             max_context_len: int, chunks_host=None) -> torch.cuda.Event:
+             max_context_len: int, chunks_host=None, positions_host=None) -> torch.cuda.Event:
         """One decode step from pinned host buffers into pinned `out_host`.
 
         q_host [S, H, D]; k/v_new_host [T, Hkv, D]; slots_host int32 [T];
@@ -220,8 +278,16 @@ class DecodeEngine:
         With fused_append and T == S, slot s must be the slot of row s's newest
         position (context_lens[s] - 1); a row whose slot is not is recorded as
         CF_DEVERR_SLOT and appends nothing.
+        An engine with a rotation takes positions_host, int32 [S], of the query
+        rows, and one new token for each of them (T == S).
         """
         S, T = q_host.shape[0], k_new_host.shape[0]
+        if (positions_host is not None) != (self.rotation is not None):
+            raise ValueError("positions_host goes with a rotation")
+        if self.rotation is not None and (T != S or positions_host.shape[0] != S):
+            raise ValueError("a rotation needs a new token and a position for every query row")
+        if chunks_host is not None and self.fp8:
+            raise ops.CacheFlowError(_lib.CF_ERR_UNSUPPORTED, "prefill chunks attend over 16-bit caches")
         b = self.slots_[self.n % len(self.slots_)]
         self.n += 1
         if b.used:
@@ -231,6 +297,8 @@ class DecodeEngine:
             b.k_new[:T].copy_(k_new_host, non_blocking=True)
             b.v_new[:T].copy_(v_new_host, non_blocking=True)
             b.slots[:T].copy_(slots_host, non_blocking=True)
+            if positions_host is not None:
+                b.pos[:T].copy_(positions_host, non_blocking=True)
             nt = tables_host.shape[0]
             b.tables[:nt, : tables_host.shape[1]].copy_(tables_host, non_blocking=True)
             b.ctx[:nt].copy_(ctx_host, non_blocking=True)
@@ -244,10 +312,15 @@ class DecodeEngine:
         self.stream.wait_event(b.h2d_done)
         if b.used:
             self.stream.wait_event(b.d2h_done)  # the slot's output was copied out
-        fused = (self.fused_append or self.fp8) and chunks_host is None and T == S
+        fused = self.rotation is None and (self.fused_append or self.fp8) and chunks_host is None and T == S
         with torch.cuda.stream(self.stream):
-            if not fused:
-                if self.fp8:
+            if self.rotation is not None:
+                self._rotate_append(b.q[:S], b.k_new[:T], b.v_new[:T], b.slots[:T], b.pos[:T])
+            elif not fused:
+                if self.block_scaled:
+                    ops.reshape_and_cache_fp8_block(b.k_new[:T], b.v_new[:T], self.k, self.v, *self.kv_scales,
+                                                    b.slots[:T])
+                elif self.fp8:
                     ops.reshape_and_cache_fp8(b.k_new[:T], b.v_new[:T], self.k, self.v, b.slots[:T],
                                               *self.kv_scales)
                 else:
