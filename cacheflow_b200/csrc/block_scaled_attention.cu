@@ -7,7 +7,7 @@
 // log2 vs[b_t] up to the reference point of the running maximum, so the online
 // softmax runs on x: the products with the stored bytes are the ones that
 // dominate the output whatever the scales are, and L counts
-// 2^(x_t) / vs[b_t].  A block whose vs is 0 adds to L alone.
+// 2^(x_t) / vs[b_t].
 #include <cmath>
 #include <mutex>
 #include <type_traits>
@@ -130,6 +130,9 @@ constexpr int kVWarp = 5;
 constexpr int kMmaWarp = 6;
 constexpr int kQWarp = 7;
 constexpr float kPScale = 256.f;
+// vs enters the exponent down to 2^-60 and multiplies the weight below (zero
+// among it), so that L, which counts weights over their vs, stays in range.
+constexpr float kLeastScale = 8.67361737988403547e-19f;
 
 // e4m3 terms of a query element and of a weight: two hold a bf16's 8
 // significant bits, three an f16's 11.
@@ -332,8 +335,16 @@ __device__ __forceinline__ Cursor find_start(const Args& a, uint8_t* smem) {
       const int64_t row = n > 0 ? n + kRow : 0;
       if (b < weight(at + row)) {
         const uint32_t w = kTileWeight * n + wi;
-        const uint32_t off = (uint32_t)(b - weight(at));  // a row's tiles are far below 2^30
-        uint32_t item = off / w, tile = (off % w + kTileWeight - 1) / kTileWeight;
+        const uint64_t off64 = (uint64_t)(b - weight(at));
+        uint32_t item, tile;
+        if (off64 >> 32 == 0) {  // (a 64-bit division is a slow one)
+          item = (uint32_t)off64 / w;
+          tile = (uint32_t)off64 % w;
+        } else {
+          item = (uint32_t)(off64 / w);
+          tile = (uint32_t)(off64 % w);
+        }
+        tile = (tile + kTileWeight - 1) / kTileWeight;
         if ((whole && tile > 0) || tile >= (uint32_t)n) {
           tile = 0;
           ++item;
@@ -702,9 +713,9 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
             (cur.tile + i) * kTile + tok < cur.ctx && ((masks[s] >> (tok / kBlk)) & 1) != 0;
         const float ks = scales[s * 2 * kTileBlocks + tok / kBlk];
         const float vs = valid ? scales[s * 2 * kTileBlocks + kTileBlocks + tok / kBlk] : 1.f;
-        const bool vzero = vs == 0.f;
-        const float lv = vzero ? 0.f : __log2f(vs);
-        const float vinv = vzero ? 1.f : __fdividef(1.f, vs);
+        const float vf = vs < kLeastScale ? kLeastScale : vs;
+        const float lv = __log2f(vf);
+        const float vinv = __fdividef(1.f, vf);
         float x[N];
 #pragma unroll
         for (int c = 0; c < N; c += 16) tmem_ld16(trow + par * N + c, &x[c]);
@@ -737,7 +748,7 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
         uint16_t pairs[N / 2];
 #pragma unroll
         for (int k = 0; k < N / 2; ++k) pairs[k] = 0;
-        const float ps = vzero ? 0.f : kPScale;
+        const float ps = vs < kLeastScale ? vs * (kPScale / kLeastScale) : kPScale;
 #pragma unroll
         for (int h = 0; h < HG; h += 2) {
           uint16_t t[kT];

@@ -294,7 +294,11 @@ __device__ __forceinline__ void norm_turn(const RopeArgs& a, float (&f)[K][2 * V
 #pragma unroll
         for (int i = 0; i < 2 * V; ++i) ss = fmaf(f[k][i], f[k][i], ss);
     }
-    rs = rsqrtf(fmaf(row_sum(ss, a.lanes_log2), a.inv_dim, a.eps));
+    // rsqrtf is off by up to two units in the last place, for the whole row;
+    // a Newton step brings that below one
+    const float s = fmaf(row_sum(ss, a.lanes_log2), a.inv_dim, a.eps);
+    rs = rsqrtf(s);
+    if (rs > 0.f) rs = fmaf(0.5f * rs, fmaf(-s * rs, rs, 1.f), rs);
   }
 #pragma unroll
   for (int k = 0; k < K; ++k) {
@@ -625,14 +629,23 @@ __global__ void __launch_bounds__(kThreads, 2) rope_block_append_kernel(const __
   if (tid < 2 * kBlk) {
     sm.top[0][tid / kBlk][tid % kBlk] = 0u;
   }
+  // A token without a position in the table counts as little as one without a
+  // slot: an earlier one with its slot is stored.
+  auto live = [&](int i) {
+    const int pos = a.positions != nullptr ? a.positions[i] : 0;
+    return pos >= 0 && (a.positions == nullptr || pos < a.max_positions);
+  };
   int key = -1;
   if (tid < kBlk) {
     if (w0 + tid < T_) {
       const int64_t slot = a.slots[w0 + tid];
-      if (slot >= a.num_slots)
+      if (!live(w0 + tid)) {
+        if (a.positions[w0 + tid] >= 0) rope_error(CF_DEVERR_POSITION);
+      } else if (slot >= a.num_slots) {
         rope_error(CF_DEVERR_SLOT);
-      else if (slot >= 0)
+      } else if (slot >= 0) {
         key = (int)(slot / kBlk);
+      }
     }
     sm.key[tid] = key;
     sm.dead[tid] = 0;
@@ -660,6 +673,7 @@ __global__ void __launch_bounds__(kThreads, 2) rope_block_append_kernel(const __
   };
   auto match = [&](int i) {
     const int slot = a.slots[i], k = slot / kBlk;
+    if (!live(i)) return;
 #pragma unroll 1
     for (int l = 0; l < kBlk; ++l) {
       if (sm.lead[l] != k) continue;
@@ -699,14 +713,7 @@ __global__ void __launch_bounds__(kThreads, 2) rope_block_append_kernel(const __
   int n;
   {
     const int l = tid / kBlk, off = tid % kBlk;
-    int tok = sm.dead[l] ? -1 : sm.win[l][off];
-    if (tok >= 0 && a.positions != nullptr) {
-      const int pos = a.positions[tok];
-      if (pos < 0 || pos >= a.max_positions) {
-        if (pos >= a.max_positions) rope_error(CF_DEVERR_POSITION);
-        tok = -1;
-      }
-    }
+    const int tok = sm.dead[l] ? -1 : sm.win[l][off];
     const uint32_t there = __ballot_sync(0xffffffffu, tok >= 0);
     if (lane == 0) sm.count[warp] = __popc(there);
     __syncthreads();
@@ -1050,15 +1057,17 @@ template <typename T, int V, int K>
 cf_status launch_block(BlockArgs b, bool interleaved, cudaStream_t stream) {
   const RopeArgs& a = b.r;
   const int windows = (a.num_tokens + kBlk - 1) / kBlk;
-  // about two CTAs per SM, as many as are resident: a CTA per (window, head)
-  // for decode steps, whole windows once there are enough of them
-  const int target = 2 * sm_count();
-  int split = (target + windows - 1) / windows;
+  // Two CTAs per SM are resident.  Up to a CTA per SM a window's heads are
+  // shared among several, and the Q rows take what is left of one wave; once
+  // the windows are more than that, Q rows get up to four CTAs per SM among
+  // them (1024 decode rows of 64 / 8 heads 18 us, 28 with the others' rule;
+  // 16384 tokens of 32 / 8 heads 126 us, 131 with eight, 152 with two).
+  const int sms = sm_count();
+  const int split = sms / windows;
   b.head_split = split < 1 ? 1 : (split > a.num_kv_heads ? a.num_kv_heads : split);
   b.kv_ctas = windows * b.head_split;
-  // (16384 tokens of 32 / 8 heads 126 us with at most four Q CTAs per SM, 131
-  // with eight, 152 with two)
-  b.q_ctas = a.num_heads > 0 ? (int32_t)row_ctas(a, K == 1 ? 4 : 1, kWarps, 4 * sm_count(), {a.num_heads}) : 0;
+  const int64_t cap = b.kv_ctas <= sms ? 2 * sms - b.kv_ctas : 4 * (int64_t)sms;
+  b.q_ctas = a.num_heads > 0 ? (int32_t)row_ctas(a, K == 1 ? 4 : 1, kWarps, cap, {a.num_heads}) : 0;
   const unsigned grid = (unsigned)(b.kv_ctas + b.q_ctas);
   if constexpr (K == 1) {
     if (full_rows(a))

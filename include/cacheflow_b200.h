@@ -370,7 +370,7 @@ CF_API cf_status cf_rope_and_cache_fp8(const cf_rope_params* params, void* key_c
  * Bytes are e4m3(x / scale), to nearest even, saturating at +-448.  With
  * power-of-two scales the division is exact and storing rows anew loses
  * nothing but what falls under e4m3's smallest normal.  A new pool's scales
- * start at 0.  Rows of a block may come in any order and place of the call;
+ * start at 0; one that is not a positive finite number counts as 0.  Rows of a block may come in any order and place of the call;
  * of two tokens with one slot the later is stored (calls of more than 16384
  * tokens count as consecutive calls of 16384).  The scale arrays move with
  * their blocks: cf_copy_blocks and the other block operators take them as
@@ -397,7 +397,8 @@ CF_API cf_status cf_rope_and_cache_fp8_block(const cf_rope_params* params, void*
 
 /* Decode attention over e4m3 caches with a scale for each block and KV head:
  * K = k_scales[block, head] * stored, V = v_scales[block, head] * stored
- * (f32, finite, >= 0; [num_blocks, num_kv_heads]).  params->dtype is the type
+ * (f32, 0 to 2^60; [num_blocks, num_kv_heads]; V scales below 2^-60 lose
+ * their weights' low bits).  params->dtype is the type
  * of the query and the output (CF_F16 or CF_BF16); head_dim 128 or 256;
  * num_blocks > 0.  A row with context 0 gives zeros.  The workspace is
  * optional: with at least cf_paged_attention_fp8_block_workspace_size() bytes

@@ -73,9 +73,8 @@ def append_block(x, cache, scales, slots, live=None):
     pool and tokens that are not `live` append nothing."""
     rows = {}
     for t, s in enumerate(slots):
-        if 0 <= s < cache.shape[0] * 16:
+        if 0 <= s < cache.shape[0] * 16 and (live is None or live[t]):
             rows[(s // 16, s % 16)] = t
-    rows = {k: t for k, t in rows.items() if live is None or live[t]}
     for b in sorted({k[0] for k in rows}):
         offs = {o: t for (bb, o), t in rows.items() if bb == b}
         for h in range(cache.shape[1]):

@@ -151,6 +151,21 @@ def test_scales_far_apart(cflib, dtype):
     _check(dtype, case, _run(dtype, case))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_scales_at_the_ends_of_their_range(cflib, dtype):
+    """Rows that begin with blocks of the least scales (a block of f32's
+    smallest values has 2^-126) and go on with ordinary ones; 2^60 beside 1."""
+    case = _case(dtype, 8, 2, 128, [700, 300, 140], seed=14)
+    q, kc, vc, ks, vs, tables, lens = case
+    vs[tables[0, :16]] = 2.0 ** -126
+    vs[tables[0, 20]] = 2.0 ** -75
+    vs[tables[1, :19]] = 2.0 ** -60
+    vs[tables[2, 3]] = 2.0 ** 60
+    if dtype == "f16":
+        vs[tables[2, 3]] = 2.0 ** 4  # (2^60 is infinity in f16)
+    _check(dtype, case, _run(dtype, case))
+
+
 def test_bytes_outside_the_context_do_not_matter(cflib):
     """NaN bytes and scales past each row's last token and in unused blocks."""
     case = _case("bf16", 8, 2, 128, [1, 15, 130, 257], seed=5, spare=4)

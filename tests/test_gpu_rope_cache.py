@@ -475,6 +475,34 @@ def test_rope_and_cache_fp8_block(cflib, dtype, H, Hkv, D, R, il):
         assert (e <= 2.0 ** -4 * np.maximum(np.abs(y[t]), 2.0 ** -6 * s) + bound[t]).all()
 
 
+def test_padding_tokens_do_not_hide_a_slot(cflib):
+    """Padding rows that all name a slot of a real token, before and after it,
+    near and far in the call: the real token is stored."""
+    import torch
+
+    from cacheflow_b200 import ops
+
+    rng = np.random.default_rng(15)
+    T, H, Hkv, D, pool = 100, 2, 2, 64, 6
+    table, table_h = _table(rng, 50, D)
+    pos = np.full(T, -1, np.int32)
+    slots = np.full(T, 35, np.int32)  # every padding row names slot 35
+    for t, s, p in ((40, 35, 7), (41, 36, 8), (10, 0, 3), (95, 1, 4)):
+        pos[t], slots[t] = p, s
+    slots[60:70] = 0
+    codes, scales = _block_state(rng, pool, Hkv, D)
+    dev = _block_device(codes, scales)
+    q, k, v = (torch.from_numpy(rng.standard_normal((T, n, D)).astype(np.float32)).cuda() for n in (H, Hkv, Hkv))
+    ops.rope_and_cache_fp8_block(q, q, k, v, *dev, torch.from_numpy(slots).cuda(), torch.from_numpy(pos).cuda(), table)
+    live = pos >= 0
+    ref.append_block(v.double().cpu().numpy(), codes[1], scales[1], slots, live)
+    _same_block([dev[1], dev[1], dev[3], dev[3]], [codes[1]] * 2, [scales[1]] * 2)
+    y = ref.norm_rope(k.double().cpu().numpy(), None, table_h, np.maximum(pos, 0), False, EPS)
+    ref.append_block(y, codes[0], scales[0], slots, live)
+    assert np.array_equal(dev[2].cpu().numpy(), scales[0])
+    assert ops.device_errors(0) == 0
+
+
 def test_scales_move_with_their_blocks(cflib):
     """copy_blocks, compact_kv_cache, memset_blocks and swap_blocks take the
     scale arrays as caches of one element a head."""
