@@ -230,11 +230,15 @@ cf_status check_rope_params(const cf_rope_params* p, bool with_cache) {
       bad(p->positions, 4) || bad(p->query_weight, wb) || bad(p->key_weight, wb) ||
       bad(with_cache ? p->value : p->key_out, eb))
     return CF_ERR_INVALID_ARGUMENT;
-  // no two rows of an output may meet (a stride of one row count is never used)
+  // no two rows of an output may meet: one of its strides steps over a row,
+  // the other over all of that one's (a stride of a count of one is not used)
   auto apart = [&](const int64_t* stride, int64_t heads) {
-    const bool h = heads == 1 || stride[1] >= p->head_dim || stride[1] <= -(int64_t)p->head_dim;
-    const bool t = p->num_tokens == 1 || stride[0] >= p->head_dim || stride[0] <= -(int64_t)p->head_dim;
-    return h && t;
+    auto width = [](int64_t x) { return x < 0 ? -(__int128)x : (__int128)x; };
+    const __int128 t = width(stride[0]), h = width(stride[1]), d = p->head_dim;
+    auto nested = [&](__int128 inner, int64_t n, __int128 outer, int64_t m) {
+      return (n == 1 || inner >= d) && (m == 1 || outer >= d + (n == 1 ? 0 : (n - 1) * inner));
+    };
+    return nested(h, heads, t, p->num_tokens) || nested(t, p->num_tokens, h, heads);
   };
   if (!apart(p->query_out_stride, p->num_heads)) return CF_ERR_INVALID_ARGUMENT;
   if (!with_cache && !apart(p->key_out_stride, p->num_kv_heads)) return CF_ERR_INVALID_ARGUMENT;

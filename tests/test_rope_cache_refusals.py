@@ -47,6 +47,24 @@ def test_rope_refusals(cflib, over, status):
     assert cflib.cf_qk_norm_rope(None, None) == BAD
 
 
+@pytest.mark.parametrize("stride,tokens,ok", [
+    ((128, 128), 4, False),    # a token's second head is the next token's first
+    ((256, 128), 4, False), ((511, 128), 4, False), ((512, 128), 4, True), ((-512, 128), 4, True),
+    ((512, -128), 4, True), ((128, 512), 4, True), ((128, 500), 4, False),  # heads outermost
+    ((0, 128), 1, True), ((128, 0), 1, False), ((2 ** 63 - 1, 128), 4, True), ((-2 ** 63, 128), 4, True),
+])
+def test_output_rows_that_meet_are_refused(cflib, stride, tokens, ok):
+    """Four heads of 128 columns.  What passes gets as far as the missing GPU."""
+    import torch
+
+    from cacheflow_b200 import _lib
+
+    if ok and torch.cuda.is_available():
+        pytest.skip("would launch")
+    st = cflib.cf_qk_norm_rope(ctypes.byref(_rope(_lib, query_out_stride=stride, num_tokens=tokens)), None)
+    assert (st != BAD) if ok else (st == BAD)
+
+
 def test_empty_calls_do_nothing(cflib):
     from cacheflow_b200 import _lib
 
