@@ -79,7 +79,7 @@ class DecodeEngine:
         if kernel not in ("v1", "reference"):
             raise ValueError("kernel must be 'v1' or 'reference'")
         self.rotation = rotation
-        self.block_scaled = kv_scales is not None and isinstance(kv_scales[0], torch.Tensor)
+        self.block_scaled = kv_scales is not None and isinstance(kv_scales[0], torch.Tensor) and kv_scales[0].dim() == 2
         if self.block_scaled and (kernel != "v1" or fused_append or key_cache.dtype != torch.float8_e4m3fn):
             raise ValueError("block scales: float8_e4m3fn caches, kernel='v1', fused_append=False")
         if rotation is not None and fused_append:
@@ -221,8 +221,6 @@ class DecodeEngine:
         decode rows (HBM-bound) on a high-priority side stream forked from it
         and joined back into it, so the decode CTAs take SMs as the prefill's
         retire instead of waiting for the whole prefill grid."""
-        if self.fp8:
-            raise ops.CacheFlowError(_lib.CF_ERR_UNSUPPORTED, "prefill chunks attend over 16-bit caches")
         nd, nc, max_q = chunks
         cur = torch.cuda.current_stream(self.device)
         if nd:
@@ -240,6 +238,11 @@ class DecodeEngine:
             cur.wait_event(self.joined)
         self.launches_per_step += 1
 
+    def _check_chunks(self, num_chunks: int) -> None:
+        """Before anything of a step is enqueued."""
+        if self.fp8 and num_chunks > 0:
+            raise ops.CacheFlowError(_lib.CF_ERR_UNSUPPORTED, "prefill chunks attend over 16-bit caches")
+
     def attend(self, num_seqs: int, max_context_len: int, chunks=None, new=None, positions=None) -> None:
         """Attention over inputs already in self.q / self.tables / self.ctx
         (the device-resident path), output in self.out; current stream.
@@ -251,6 +254,8 @@ class DecodeEngine:
         [num_seqs]) are of every query row, and self.q is rotated in place."""
         S = num_seqs
         extra = 0
+        if chunks is not None:
+            self._check_chunks(chunks[1])
         if self.rotation is not None:
             if new is None or positions is None:
                 raise ValueError("a rotation needs the new tokens and their positions")
@@ -286,8 +291,8 @@ class DecodeEngine:
             raise ValueError("positions_host goes with a rotation")
         if self.rotation is not None and (T != S or positions_host.shape[0] != S):
             raise ValueError("a rotation needs a new token and a position for every query row")
-        if chunks_host is not None and self.fp8:
-            raise ops.CacheFlowError(_lib.CF_ERR_UNSUPPORTED, "prefill chunks attend over 16-bit caches")
+        if chunks_host is not None:
+            self._check_chunks(chunks_host[2].shape[0])
         b = self.slots_[self.n % len(self.slots_)]
         self.n += 1
         if b.used:

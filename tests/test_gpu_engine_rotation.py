@@ -148,3 +148,90 @@ def test_refusals(cflib):
     e8 = DecodeEngine(c8, c8.clone(), 4, 2, 4, kv_scales=(sc, sc), query_dtype=torch.bfloat16)
     with pytest.raises(ops.CacheFlowError):  # prefill chunks take 16-bit caches
         e8.step(q, k, k, i, torch.zeros(2, 4, dtype=torch.int32), i, q.clone(), 1, chunks_host=(1, i, i[:1], i[None]))
+
+
+def test_refused_chunks_leave_the_cache_alone(cflib):
+    """Chunks over an 8-bit cache are refused before anything is rotated or appended; a step that has none is not."""
+    import torch
+
+    from cacheflow_b200 import ops
+    from cacheflow_b200.engine import DecodeEngine, Rotation
+
+    rng = np.random.default_rng(8)
+    c8 = torch.zeros(2, 4, 2, 16, 128, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    sc = torch.zeros(2, 4, 2, device="cuda")
+    eng = DecodeEngine(c8[0], c8[1], 4, 2, 4, kv_scales=(sc[0], sc[1]), query_dtype=torch.bfloat16,
+                       rotation=Rotation(ops.rope_table(64, 128)), max_chunks=1)
+    q, k, v = (torch.from_numpy(rng.standard_normal(s).astype(np.float32)).bfloat16().pin_memory()
+               for s in ((2, 4, 128), (2, 2, 128), (2, 2, 128)))
+    slots, pos, ctx, start = (torch.tensor(x, dtype=torch.int32).pin_memory() for x in ([0, 16], [0, 0], [1, 1], [0, 0]))
+    tables = torch.tensor([[0, 0, 0, 0], [1, 0, 0, 0]], dtype=torch.int32).pin_memory()
+    new = (k.cuda(), v.cuda(), slots.cuda())
+    eng.q.copy_(q)
+    with pytest.raises(ops.CacheFlowError):
+        eng.attend(2, 1, chunks=(1, 1, 1), new=new, positions=pos.cuda())
+    torch.cuda.synchronize()
+    assert torch.equal(eng.q.cpu(), q) and not c8.view(torch.uint8).any() and not sc.any()
+    out = torch.zeros(2, 4, 128, dtype=torch.bfloat16).pin_memory()
+    # no chunk: both rows decode; at position 0 a row's output is its own V
+    eng.step(q, k, v, slots, tables, ctx, out, 1, chunks_host=(2, start[:1], ctx[:0], tables[:0]),
+             positions_host=pos)
+    eng.synchronize()
+    want = v.double().repeat_interleave(2, 1)
+    assert (out.double() - want).abs().max() <= 2.0 ** -4 * (1 + 2.0 ** -7) * want.abs().max()
+    assert sc.all(2)[:, :2].all() and ops.device_errors(0) == 0
+
+
+def test_rotation_with_prefill_chunks(cflib):
+    """A decode row and a chunk of a prompt in one step: as rope_and_cache and the two attentions in turn."""
+    import torch
+
+    from cacheflow_b200 import ops
+    from cacheflow_b200.engine import DecodeEngine, Rotation
+
+    rng = np.random.default_rng(4)
+    H, Hkv, D, n = 8, 2, 128, 21
+    S = n + 1
+    kc, vc = (torch.zeros(8, Hkv, 16, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    k2, v2 = kc.clone(), vc.clone()
+    rot = Rotation(ops.rope_table(64, D))
+    eng = DecodeEngine(kc, vc, H, S, 2, rotation=rot, max_chunks=1)
+    q, k, v = (torch.from_numpy(rng.standard_normal(s).astype(np.float32)).bfloat16().pin_memory()
+               for s in ((S, H, D), (S, Hkv, D), (S, Hkv, D)))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32).pin_memory()  # noqa: E731
+    tables = i32([[5, 0]] + [[2, 7]] * n)
+    pos = i32([0] + list(range(n)))
+    slots = i32([80] + [(2, 7)[p // 16] * 16 + p % 16 for p in range(n)])
+    out = torch.empty(S, H, D, dtype=torch.bfloat16).pin_memory()
+    chunk = (1, i32([0, n]), i32([n]), tables[1:2])
+    eng.step(q, k, v, slots, tables, pos + 1, out, n, chunks_host=chunk, positions_host=pos)
+    eng.synchronize()
+    qd, want = q.cuda(), torch.empty(S, H, D, dtype=torch.bfloat16, device="cuda")
+    ops.rope_and_cache(qd, qd, k.cuda(), v.cuda(), k2, v2, slots.cuda(), pos.cuda(), rot.cos_sin)
+    ops.paged_attention_v1(want[:1], qd[:1], k2, v2, tables[:1].cuda(), i32([1]).cuda(), None, 1)
+    ops.paged_prefill_attention(want[1:], qd[1:], k2, v2, tables[1:2].cuda(), i32([n]).cuda(), i32([0, n]).cuda(),
+                                None, n)
+    assert torch.equal(kc, k2) and torch.equal(vc, v2)
+    # the decode row attends to itself alone and the chunk's launch is the same one
+    assert torch.equal(out, want.cpu())
+    assert ops.device_errors(0) == 0
+
+
+def test_scales_given_as_scalar_tensors(cflib):
+    """A scale for a whole cache may still be a tensor of one number."""
+    import torch
+
+    from cacheflow_b200.engine import DecodeEngine
+
+    outs = []
+    for scales in ((0.5, 0.25), (torch.tensor(0.5), torch.tensor([0.25]))):
+        c8 = torch.zeros(2, 4, 2, 16, 128, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+        eng = DecodeEngine(c8[0], c8[1], 4, 2, 4, kv_scales=scales, query_dtype=torch.bfloat16)
+        g = torch.Generator().manual_seed(3)
+        q, k, v = (torch.randn(s, generator=g).bfloat16().pin_memory() for s in ((1, 4, 128), (1, 2, 128), (1, 2, 128)))
+        one = torch.ones(1, dtype=torch.int32).pin_memory()
+        out = torch.empty(1, 4, 128, dtype=torch.bfloat16).pin_memory()
+        eng.step(q, k, v, one * 0, one[:, None] * 0, one, out, 1)
+        eng.synchronize()
+        outs.append(out)
+    assert torch.equal(*outs) and outs[0].any()
