@@ -417,8 +417,8 @@ def _rope_params(q_out, query, key, positions, cos_sin, q_weight, k_weight, eps,
         packed = _ROPE_PARAMS.pack(q, k, v, qo, ko, positions.data_ptr(), cos_sin.data_ptr(), qw, kw, q0, q1, k0, k1,
                                    v0, v1, qo0, qo1, ko0, ko1, T, H, ks[1], D, ts[1], ts[0], eps,
                                    1 if interleaved else 0, code, wcode)
-    except struct.error as e:
-        raise _bad(f"a size does not fit 32 bits: {e}") from None
+    except (struct.error, OverflowError) as e:
+        raise _bad(f"a size or number does not fit 32 bits: {e}") from None
     return _lib.RopeParams.from_buffer_copy(packed), dev
 
 
@@ -514,6 +514,8 @@ def reshape_and_cache_fp8_block(key, value, key_cache, value_cache, k_scales, v_
     v, v0, v1 = _rows("value", value, shape, key.dtype, dev)
     if (k1 != D or v1 != D) and Hkv > 1:
         raise _bad("key/value: a token's heads must be contiguous")
+    if T > 0x7fffffff:
+        raise _bad("num_tokens does not fit 32 bits")
     blocks, size = _check_caches(key_cache, value_cache, key, torch.float8_e4m3fn, slot_mapping, dev)
     _check_scales(k_scales, v_scales, key_cache, dev)
     _call(lib.cf_reshape_and_cache_fp8_block, dev, "cf_reshape_and_cache_fp8_block", k, v, key_cache.data_ptr(),
@@ -562,8 +564,8 @@ def paged_attention_fp8_block_v1(out, query, key_cache, value_cache, k_scales, v
         packed = _ATTENTION_PARAMS.pack(query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), out.data_ptr(),
                                         block_tables.data_ptr(), context_lens.data_ptr(), scale, qs[0], qs[1], cs[1],
                                         qs[2], cs[2], max_context_len, bs[1], cs[0], dtype_code(dt))
-    except struct.error as e:
-        raise _bad(f"a size does not fit 32 bits: {e}") from None
+    except (struct.error, OverflowError) as e:
+        raise _bad(f"a size or number does not fit 32 bits: {e}") from None
     p = AttentionParams.from_buffer_copy(packed)
     ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(),
                                                         workspace.numel() * workspace.element_size())

@@ -587,3 +587,20 @@ def test_on_a_stream_and_captured(cflib):
     # stored in e4m3: each value off by up to 2^-4, 2.6e-2 of it on the mean square
     assert np.linalg.norm(got - want) / np.linalg.norm(want) < 0.06
     assert ops.device_errors(0) == 0
+
+
+def test_numbers_past_f32_are_refused(cflib):
+    import torch
+
+    from cacheflow_b200 import ops
+
+    q = torch.zeros(2, 4, 128, dtype=torch.bfloat16, device="cuda")
+    pos = torch.zeros(2, dtype=torch.int32, device="cuda")
+    w = torch.ones(128, device="cuda")
+    for eps in (1e300, float("inf"), 0.0):
+        with pytest.raises(ops.CacheFlowError):
+            ops.qk_norm_rope(q, q.clone(), q, q.clone(), pos, ops.rope_table(8, 128), w, w, eps=eps)
+    c8 = torch.zeros(2, 4, 16, 128, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    sc = torch.zeros(2, 4, device="cuda")
+    with pytest.raises(ops.CacheFlowError):
+        ops.paged_attention_fp8_block_v1(q.clone(), q, c8, c8, sc, sc, pos[:, None], pos, scale=1e300)
