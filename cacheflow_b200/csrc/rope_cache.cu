@@ -21,8 +21,8 @@
 // tokens of 32 / 8 heads with the append 86 us, 4.75 TB/s; 4095 f32 tokens of
 // 32 / 32 heads of 64 27 us, 5.05 TB/s.  A decode step of 64 rows is launch
 // latency, 4.3 us.  The block-scaled append is bound by its CTAs' chain of
-// dependent steps instead: 16384 tokens of 32 / 8 heads in ragged prompts 128
-// us, 2.95 TB/s; 1024 decode rows of 64 / 8 heads 18 us.
+// dependent steps instead: 16384 tokens of 32 / 8 heads in ragged prompts 117
+// us, 3.23 TB/s; 1024 decode rows of 64 / 8 heads 18 us.
 #include <atomic>
 #include <initializer_list>
 #include <mutex>
@@ -580,6 +580,7 @@ struct BlockSmem {
   int32_t dead[kBlk];           // its first token lies before the window
   int32_t win[kBlk][kBlk];      // token that gives row `off` of block lead[l], -1: none
   uint32_t filter[32];
+  uint32_t few[2];              // first slots of the first two blocks led
   int32_t row_tok[kBlk * kBlk]; // the rows to append: token, and l * 16 + off
   int32_t row_lo[kBlk * kBlk];
   int32_t count[kWarps];
@@ -635,16 +636,15 @@ __global__ void __launch_bounds__(kThreads, 2) rope_block_append_kernel(const __
   }
   // A token without a position in the table counts as little as one without a
   // slot: an earlier one with its slot is stored.
-  auto live = [&](int i) {
-    const int pos = a.positions != nullptr ? a.positions[i] : 0;
-    return pos >= 0 && (a.positions == nullptr || pos < a.max_positions);
-  };
+  auto position = [&](int i) { return a.positions != nullptr ? a.positions[i] : 0; };
+  auto live = [&](int pos) { return pos >= 0 && pos < a.max_positions; };
   int key = -1;
   if (tid < kBlk) {
     if (w0 + tid < T_) {
       const int64_t slot = a.slots[w0 + tid];
-      if (!live(w0 + tid)) {
-        if (a.positions[w0 + tid] >= 0) rope_error(CF_DEVERR_POSITION);
+      const int pos = position(w0 + tid);
+      if (!live(pos)) {
+        if (pos >= 0) rope_error(CF_DEVERR_POSITION);
       } else if (slot >= a.num_slots) {
         rope_error(CF_DEVERR_SLOT);
       } else if (slot >= 0) {
@@ -663,21 +663,29 @@ __global__ void __launch_bounds__(kThreads, 2) rope_block_append_kernel(const __
     leads = key >= 0 && first == tid;
     sm.lead[tid] = leads ? key : -1;
     if (leads) atomicOr(&sm.filter[(key >> 5) & 31], 1u << (key & 31));
+    const uint32_t leaders = __ballot_sync(0xffffu, leads);
+    const int before = __popc(leaders & ((1u << tid) - 1u));
+    if (leads && before < 2) sm.few[before] = (uint32_t)key * kBlk;
+    if (leads && leaders == 1u << tid) sm.few[1] = (uint32_t)key * kBlk;
     if (key >= 0) atomicMax(&sm.win[first][a.slots[w0 + tid] % kBlk], w0 + tid);
   }
-  if (__syncthreads_or(leads ? 1 : 0) == 0) return;  // padding only
+  const int led = __syncthreads_count(leads ? 1 : 0);
+  if (led == 0) return;  // padding only
 
   // 2. their tokens outside the window, wherever they are in the call (seldom
   // more than a run that goes on behind it): four slots a load where they are
-  // 16-byte aligned, eight loads in flight (16384 slots one at a time and 16 in
-  // flight took 5.3 us of a CTA's 17)
+  // 16-byte aligned, eight loads in flight.  One or two blocks, as a window of
+  // a prompt has, are compared with directly, more of them looked up in the
+  // filter (16384 tokens of prompts, 32 / 8 heads: 117 us, 127 with the filter
+  // for all; looking up four slots for one bit took 1024 decode rows from 18
+  // to 22 us, by the false hits).
   auto hit = [&](int slot) -> uint32_t {
     const int k = slot / kBlk;
     return slot >= 0 ? (sm.filter[(k >> 5) & 31] >> (k & 31)) & 1u : 0u;
   };
   auto match = [&](int i) {
     const int slot = a.slots[i], k = slot / kBlk;
-    if (!live(i)) return;
+    if (slot < 0 || !live(position(i))) return;
 #pragma unroll 1
     for (int l = 0; l < kBlk; ++l) {
       if (sm.lead[l] != k) continue;
@@ -699,9 +707,17 @@ __global__ void __launch_bounds__(kThreads, 2) rope_block_append_kernel(const __
       slot[u] = look ? reinterpret_cast<const int4*>(a.slots)[q] : make_int4(-1, -1, -1, -1);
     }
     uint32_t hits = 0u;
+    if (led <= 2) {
+      const uint32_t lo0 = sm.few[0], lo1 = sm.few[1];
+      auto in = [&](int x) { return (uint32_t)x - lo0 < (uint32_t)kBlk || (uint32_t)x - lo1 < (uint32_t)kBlk; };
 #pragma unroll
-    for (int u = 0; u < kLook; ++u)
-      hits |= (hit(slot[u].x) | hit(slot[u].y) << 1 | hit(slot[u].z) << 2 | hit(slot[u].w) << 3) << (4 * u);
+      for (int u = 0; u < kLook; ++u)
+        if (in(slot[u].x) || in(slot[u].y) || in(slot[u].z) || in(slot[u].w)) hits |= 15u << (4 * u);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kLook; ++u)
+        hits |= (hit(slot[u].x) | hit(slot[u].y) << 1 | hit(slot[u].z) << 2 | hit(slot[u].w) << 3) << (4 * u);
+    }
 #pragma unroll 1
     for (; hits != 0u; hits &= hits - 1u) {
       const int j = __ffs(hits) - 1;
@@ -1065,7 +1081,8 @@ cf_status launch_block(BlockArgs b, bool interleaved, cudaStream_t stream) {
   // shared among several, and the Q rows take what is left of one wave; once
   // the windows are more than that, Q rows get up to four CTAs per SM among
   // them (1024 decode rows of 64 / 8 heads 18 us, 28 with the others' rule;
-  // 16384 tokens of 32 / 8 heads 126 us, 131 with eight, 152 with two).
+  // 16384 tokens of 32 / 8 heads 126 us, 131 with eight, 152 with two, before
+  // the search took what it takes now).
   const int sms = sm_count();
   const int split = sms / windows;
   b.head_split = split < 1 ? 1 : (split > a.num_kv_heads ? a.num_kv_heads : split);
@@ -1172,7 +1189,10 @@ cf_status launch_rope_and_cache_fp8_block(const cf_rope_params& p, void* key_cac
     a.v = at(a.v, a.v_ts);
     a.q_out = at(a.q_out, a.qo_ts);
     a.k_out = nullptr;
-    a.positions = a.positions == nullptr ? nullptr : a.positions + t0;
+    if (a.positions != nullptr)
+      a.positions += t0;
+    else
+      a.max_positions = 1;  // every token's position counts as 0
     a.num_tokens = (int32_t)(p.num_tokens - t0 < kPiece ? p.num_tokens - t0 : kPiece);
     a.dest = kCacheFp8;
     a.kc = key_cache;

@@ -604,3 +604,47 @@ def test_numbers_past_f32_are_refused(cflib):
     sc = torch.zeros(2, 4, device="cuda")
     with pytest.raises(ops.CacheFlowError):
         ops.paged_attention_fp8_block_v1(q.clone(), q, c8, c8, sc, sc, pos[:, None], pos, scale=1e300)
+
+
+@pytest.mark.parametrize("blocks", [1, 2, 3])
+@pytest.mark.parametrize("op", ["append", "rope"])
+def test_block_append_of_rows_far_from_their_window(cflib, blocks, op):
+    """A window that leads one, two or three blocks, block 0 among them, whose
+    other rows, some of them twice, lie anywhere in the call, beside padding
+    with every negative slot and tokens whose positions are out of the table."""
+    import torch
+
+    from cacheflow_b200 import ops
+
+    rng = np.random.default_rng(60 + blocks)
+    T, Hkv, D, pool = 600, 2, 128, 40
+    ids = [0, 7, 39][:blocks]
+    slots = -rng.integers(1, 40, T).astype(np.int32)
+    rest = rng.permutation([b for b in range(pool) if b not in ids])
+    slots[16:32] = [ids[i % blocks] * 16 + i // blocks % 3 for i in range(16)]
+    for i in rng.choice(np.arange(48, T), 60, replace=False):
+        slots[i] = ids[rng.integers(blocks)] * 16 + rng.integers(16)
+    for n, i in enumerate(rng.choice(np.flatnonzero(slots < 0), 200, replace=False)):
+        slots[i] = rest[n % 30] * 16 + rng.integers(16)
+    pos = rng.integers(0, 50, T).astype(np.int32)
+    if op == "rope":
+        pos[rng.random(T) < 0.1] = -1
+    x = rng.standard_normal((2, T, Hkv, D)).astype(np.float32)
+    codes, sc = np.zeros((2, pool, Hkv, 16, D), np.uint8), np.zeros((2, pool, Hkv), np.float32)
+    dev = _block_device(codes, sc)
+    k, v = (torch.from_numpy(a).bfloat16().cuda() for a in x)
+    s, p = torch.from_numpy(slots).cuda(), torch.from_numpy(pos).cuda()
+    want = slots.copy()
+    if op == "append":
+        ops.reshape_and_cache_fp8_block(k, v, *dev, s)
+    else:
+        table = torch.cat([torch.ones(50, D // 2), torch.zeros(50, D // 2)], 1).cuda()  # angles of zero
+        q = torch.zeros(T, 1, D, dtype=torch.bfloat16, device="cuda")
+        ops.rope_and_cache_fp8_block(q, q, k, v, *dev, s, p, table)
+        want[pos < 0] = -1
+    for i, t in enumerate((k, v)):
+        ref.append_block(t.double().cpu().numpy(), codes[i], sc[i], want)
+    assert np.array_equal(dev[0].view(torch.uint8).cpu().numpy(), codes[0])
+    assert np.array_equal(dev[1].view(torch.uint8).cpu().numpy(), codes[1])
+    assert np.array_equal(dev[2].cpu().numpy(), sc[0]) and np.array_equal(dev[3].cpu().numpy(), sc[1])
+    assert ops.device_errors(0) == 0
