@@ -4,10 +4,11 @@
 // over t < context_lens[s], b_t the block of token t.
 //
 // A weight p_t vs[b_t] is 2^(x_t) / L with x_t = log2(e) scale ks q.k_t +
-// log2 vs[b_t] up to the reference point of the running maximum, so the online
-// softmax runs on x: the products with the stored bytes are the ones that
-// dominate the output whatever the scales are, and L counts
-// 2^(x_t) / vs[b_t].
+// log2 vs[b_t] up to a reference point, so the online softmax runs on x: the
+// products with the stored bytes are the ones that dominate the output
+// whatever the scales are, and L counts 2^(x_t) / vs[b_t].  A tile's weights
+// are taken from the tile's own maximum and its sums join the row's in f32, so
+// what a weight loses to its 8-bit terms goes by its tile, not by its row.
 #include <cmath>
 #include <mutex>
 #include <type_traits>
@@ -110,8 +111,17 @@ struct Cursor {
 // would round to 4 bits, are two or three e4m3 terms each, in as many of the
 // N columns per head: x = t1 + t2 / 16 + t3 / 256, every term the rounding of
 // 16 times what the ones before it leave.  Q is brought under 448 by a power
-// of two for each head, P lies in [0, 256].  The block scales join outside:
-// ks on a token's logit, vs in its weight's exponent.
+// of two for each head, P is 256 at the tile's maximum.  The block scales join
+// outside: ks on a token's logit, vs in its weight's exponent.
+//
+// Rounding: Q's terms hold every bit of a bf16 (an f16 to 2^-12).  P's are
+// off by 2^-8 p at most (f16 2^-11) from 2^-14 of the tile's largest on, and
+// below by 2^-22 (2^-26) of that one: as much as a P rounded to the rows' type
+// but for tokens that next to nothing is left for in their tile.  The sum L
+// has the weights before they are rounded.  With the row's running maximum as
+// the reference the rest of a row with one dominant token fell under that
+// floor as a whole (131072 tokens with 1 % of the weight beside one: 60-84 %
+// of the output lost).
 //
 // Roles: warps 4 and 5 issue the TMA copies of K and of V (2 KB boxes of 16
 // tokens x 128 bytes, 128-byte swizzle) into rings of stages, warp 7 stages
@@ -119,7 +129,7 @@ struct Cursor {
 // warps 0-3 do the softmax: thread t has token t of each tile, reads its
 // logit terms from tensor memory, and writes its P bytes; as the owner of
 // head dimension t it reads the tile's O from tensor memory and adds it to
-// f32 registers, rescaled there when the maximum moved.  The copies run on
+// f32 registers, both brought to the larger maximum.  The copies run on
 // across segments, QK runs two tiles ahead of PV (S is double-buffered), and
 // a tile's PV runs under the next tile's logits, whose warps add its O while
 // they wait for each other's maxima.
@@ -137,6 +147,7 @@ constexpr int kVWarp = 5;
 constexpr int kMmaWarp = 6;
 constexpr int kQWarp = 7;
 constexpr float kPScale = 256.f;
+constexpr float kNoMax = -3.402823466e38f;  // the maximum over no token: finite, so that differences are
 // vs enters the exponent down to 2^-60 and multiplies the weight below (zero
 // among it), so that L, which counts weights over their vs, stays in range.
 constexpr float kLeastScale = 8.67361737988403547e-19f;
@@ -679,16 +690,15 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
     for (int seg = 0; !cur.done(); cur.next(a), ++seg) {
       const int cnt = cur.count();
       const int kvh = cur.item / a.head_chunks, chunk = cur.item - kvh * a.head_chunks;
-      float qsc[HG], m[HG], l[HG], alpha[HG], acc[L::kBoxes][HG];
+      float qsc[HG], m[HG], l[HG], beta[HG], acc[L::kBoxes][HG];
       if (warp == 0 && !wait_bar(q_full, (uint32_t)seg & 1u, a.wait_limit_ns)) *fail = 1;
       ok = meet();
       if (!ok) break;
 #pragma unroll
       for (int h = 0; h < HG; ++h) {
         qsc[h] = sqs[h] * a.scale_log2;
-        m[h] = -INFINITY;
+        m[h] = kNoMax;
         l[h] = 0.f;
-        alpha[h] = 0.f;
 #pragma unroll
         for (int b = 0; b < L::kBoxes; ++b) acc[b][h] = 0.f;
       }
@@ -705,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
           for (int c = 0; c < N; c += 16) tmem_ld16(trow + L::kOCol + b * N + c, &o[c]);
           tmem_wait_ld();
 #pragma unroll
-          for (int h = 0; h < HG; ++h) acc[b][h] = fmaf(acc[b][h], alpha[h], join_terms<kT, HG>(o, h));
+          for (int h = 0; h < HG; ++h) acc[b][h] = fmaf(join_terms<kT, HG>(o, h), beta[h], acc[b][h]);
         }
       };
       for (int i = 0; i < cnt; ++i, ++j) {
@@ -742,14 +752,18 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
         if (!ok) break;
 #pragma unroll
         for (int h = 0; h < HG; ++h) {
-          const float mx = fmaxf(fmaxf(tops[h], tops[L::kMaxHeads + h]),
+          const float mx = fmaxf(fmaxf(fmaxf(tops[h], tops[L::kMaxHeads + h]), kNoMax),
                                  fmaxf(tops[2 * L::kMaxHeads + h], tops[3 * L::kMaxHeads + h]));
-          const float mn = fmaxf(m[h], mx);
-          const float mu = mn == -INFINITY ? 0.f : mn;
-          alpha[h] = ex2_approx(m[h] - mu);
-          m[h] = mn;
-          x[h] = ex2_approx(x[h] - mu);
-          l[h] = fmaf(l[h], alpha[h], x[h] * vinv);
+          // of 2^(m - max) and 2^(mx - max), which bring the row's sums and the
+          // tile's to the larger of the two maxima, one is 1
+          const float d = m[h] - mx, r = ex2_approx(-fabsf(d));
+          const float alpha = d < 0.f ? r : 1.f;
+          beta[h] = d < 0.f ? 1.f : r;
+          m[h] = fmaxf(m[h], mx);
+          x[h] = ex2_approx(x[h] - mx);
+          l[h] = fmaf(x[h] * vinv, beta[h], l[h] * alpha);
+#pragma unroll
+          for (int b = 0; b < L::kBoxes; ++b) acc[b][h] *= alpha;
         }
         // P's bytes: column t HG + h is term t of head h
         uint16_t pairs[N / 2];
@@ -879,7 +893,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) block_attention_join_kernel(c
       const int mine = p0 + stride * lane;
       const float sum = mine < pieces ? a.part_sum[slot(mine)] : 0.f;
       const float top = mine < pieces ? a.part_max[slot(mine)] : -INFINITY;
-      // a piece without a readable token has sum 0 and maximum -inf
+      // a piece without a readable token has sum 0
       const float mn = fmaxf(m, warp_max(top));
       const float mu = mn == -INFINITY ? 0.f : mn;
       const float alpha = exp2f(m - mu);

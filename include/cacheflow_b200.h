@@ -398,7 +398,9 @@ CF_API cf_status cf_rope_and_cache_fp8_block(const cf_rope_params* params, void*
 /* Decode attention over e4m3 caches with a scale for each block and KV head:
  * K = k_scales[block, head] * stored, V = v_scales[block, head] * stored
  * (f32, 0 to 2^60; [num_blocks, num_kv_heads]; V scales below 2^-60 lose
- * their weights' low bits).  params->dtype is the type
+ * their weights' low bits).  A token's weight times its V scale is held to
+ * 2^-8 of itself (CF_F16 2^-11), or to 2^-22 (2^-26) of the largest of its 128
+ * neighbours (tokens 128 i to 128 i + 127) where that is more.  params->dtype is the type
  * of the query and the output (CF_F16 or CF_BF16); head_dim 128 or 256;
  * num_blocks > 0.  A row with context 0 gives zeros.  The workspace is
  * optional: with at least cf_paged_attention_fp8_block_workspace_size() bytes
