@@ -184,7 +184,7 @@ struct Layout {
   static constexpr int kNumBars = 4 * kStages + 2 + 5;
   static constexpr int kScaleOff = kBarOff + (kNumBars * 8 + 15) / 16 * 16;  // [stages][ks 8, vs 8] f32
   static constexpr int kMaskOff = kScaleOff + kStages * 2 * kTileBlocks * 4;  // [stages] int
-  static constexpr int kFailOff = kMaskOff + 16;                              // int: a wait ran out
+  static constexpr int kFailOff = kMaskOff + 16;                              // [2] int: a wait ran out
   static constexpr int kMaxOff = kFailOff + 16;                               // [2][4][HG] f32
   static constexpr int kMaxHeads = (HG + 3) / 4 * 4;
   static constexpr int kSumOff = kMaxOff + 2 * 4 * kMaxHeads * 4;          // [4][HG] f32
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
   uint64_t* fin = q_empty + 1;
   float* scales = reinterpret_cast<float*>(smem + L::kScaleOff);
   int* masks = reinterpret_cast<int*>(smem + L::kMaskOff);
-  volatile int* fail = reinterpret_cast<int*>(smem + L::kFailOff);  // of a softmax warp
+  volatile int* fail = reinterpret_cast<int*>(smem + L::kFailOff);  // of a softmax warp, before a meeting of either kind
   float* smax = reinterpret_cast<float*>(smem + L::kMaxOff);
   float* ssum = reinterpret_cast<float*>(smem + L::kSumOff);
   float* sqs = reinterpret_cast<float*>(smem + L::kQsOff);
@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
     mbar_init(smem_addr(q_full), 32);
     mbar_init(smem_addr(q_empty), 1 + 4);  // its last QK, and the softmax warps' reads of the scales
     mbar_init(smem_addr(fin), 1);
-    *fail = 0;
+    fail[0] = fail[1] = 0;
     fence_mbar_init();
   }
   if (warp == kMmaWarp) {
@@ -679,20 +679,23 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
     const Shares& sh = *reinterpret_cast<const Shares*>(smem + L::kSharesOff);
     int64_t at = sh.first;  // weight before the segment's item
     // Warp 0 waits for the others, which sleep at a hardware barrier: polling
-    // warps would take the issue slots of the other CTAs' softmax.  A wait
-    // that runs out sets *fail; every warp sees it after the next barrier and
-    // leaves, so the four warps meet at every barrier.
-    auto meet = [&]() {
+    // warps would take the issue slots of the other CTAs' softmax.  A wait that
+    // runs out sets fail[] of the next meeting, and every warp reads it there
+    // and leaves.  Meetings alternate between two kinds (0 and 1), so nobody
+    // sets one's flag before the others have read it at the last of its kind:
+    // the four warps leave at the same one.  (A barrier that reduces a
+    // predicate, the other way to this, takes 267 us against 250 at 256 rows.)
+    auto meet = [&](int kind) {
       asm volatile("bar.sync 1, 128;" ::: "memory");
-      return *fail == 0;
+      return fail[kind] == 0;
     };
     bool ok = true;
     for (int seg = 0; !cur.done(); cur.next(a), ++seg) {
       const int cnt = cur.count();
       const int kvh = cur.item / a.head_chunks, chunk = cur.item - kvh * a.head_chunks;
       float qsc[HG], m[HG], l[HG], beta[HG], acc[L::kBoxes][HG];
-      if (warp == 0 && !wait_bar(q_full, (uint32_t)seg & 1u, a.wait_limit_ns)) *fail = 1;
-      ok = meet();
+      if (warp == 0 && !wait_bar(q_full, (uint32_t)seg & 1u, a.wait_limit_ns)) fail[0] = 1;
+      ok = meet(0);
       if (!ok) break;
 #pragma unroll
       for (int h = 0; h < HG; ++h) {
@@ -704,8 +707,9 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_addr(q_empty));
-      auto add_o = [&](uint32_t t) {  // the accumulator takes tile t's O
-        if (!wait_bar(o_full, t & 1u, a.wait_limit_ns)) *fail = 1;
+      // the accumulator takes tile t's O, before a meeting of this kind
+      auto add_o = [&](uint32_t t, int kind) {
+        if (!wait_bar(o_full, t & 1u, a.wait_limit_ns)) fail[kind] = 1;
         __syncwarp();
         tc_fence_after();
 #pragma unroll
@@ -722,8 +726,8 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
         const int par = (int)(j & 1), s = (int)(j % S);
         if (warp == 0 && !(wait_bar(&v_full[s], (j / S) & 1u, a.wait_limit_ns) &&
                            wait_bar(&s_full[par], (j >> 1) & 1u, a.wait_limit_ns)))
-          *fail = 1;
-        ok = meet();
+          fail[1] = 1;
+        ok = meet(1);
         if (!ok) break;
         tc_fence_after();
         const bool valid =
@@ -747,8 +751,8 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
         }
         // The last tile's O, while the other warps' maxima come in.  After it
         // P and O are free: this tile's PV may write them.
-        if (i > 0) add_o(j - 1);
-        ok = meet();
+        if (i > 0) add_o(j - 1, 0);
+        ok = meet(0);
         if (!ok) break;
 #pragma unroll
         for (int h = 0; h < HG; ++h) {
@@ -806,7 +810,7 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
         mbar_arrive(smem_addr(p_full));
       }
       if (!ok) break;
-      add_o(j - 1);
+      add_o(j - 1, 1);
 
       // The segment's sums over its 128 token threads, then its result.
 #pragma unroll
@@ -816,7 +820,7 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
         for (int k = 16; k > 0; k >>= 1) w += shfl_xor(w, k);
         if (lane == 0) ssum[warp * L::kMaxHeads + h] = w;
       }
-      ok = meet();
+      ok = meet(1);
       if (!ok) break;
       const bool whole = cur.tile == 0 && cnt == cur.tiles;
       const int slot = 2 * blockIdx.x + (cur.tile == 0 ? 1 : 0);
