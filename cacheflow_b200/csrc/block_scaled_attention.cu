@@ -46,7 +46,7 @@ struct Args {
   // takes the items that begin in its tiles.
   int4* meta;        // [G]: row, KV head and chunk, last CTA of the item begun (row -1: none)
   float* part_max;   // [2 G, HG] log2 units
-  float* part_sum;
+  float* part_sum;   // kNoPiece: the CTA could not finish the piece
   float* part_out;   // [2 G, HG, D]
   float scale_log2;
   int32_t num_seqs, num_heads, num_kv_heads, group;
@@ -54,9 +54,10 @@ struct Args {
   int32_t head_chunks;  // items per (row, KV head)
   int64_t num_blocks;
   uint64_t wait_limit_ns;     // of every pipeline wait
-  int32_t unarm_first_stage;  // test hook (cf_testing_set_pipeline_faults)
+  int32_t unarm_cta;          // test hook (cf_testing_set_pipeline_faults): a CTA, kEveryCta or kNoCta
 };
 
+constexpr int kNoCta = -2, kEveryCta = -1;
 constexpr int kTile = 128;                 // tokens of a tile
 constexpr int kTileWeight = 4;             // of a tile in the shares
 constexpr int kItemWeight = 3;             // of an item's beginning and end
@@ -147,6 +148,7 @@ constexpr int kVWarp = 5;
 constexpr int kMmaWarp = 6;
 constexpr int kQWarp = 7;
 constexpr float kPScale = 256.f;
+constexpr float kNoPiece = -1.f;  // in the place of a sum
 constexpr float kNoMax = -3.402823466e38f;  // the maximum over no token: finite, so that differences are
 // vs enters the exponent down to 2^-60 and multiplies the weight below (zero
 // among it), so that L, which counts weights over their vs, stays in range.
@@ -510,7 +512,8 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
               break;
             }
           }
-          if (a.unarm_first_stage && j == 0) continue;  // test hook: the stage never completes
+          if (j == 0 && (a.unarm_cta == kEveryCta || a.unarm_cta == (int)blockIdx.x))
+            continue;  // test hook: the stage never completes
           const uint32_t bar = smem_addr(&fulls[s]);
           if (lane == 0) {
             if (!is_k) masks[s] = (int)mask;
@@ -853,6 +856,8 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
       at += (int64_t)kTileWeight * cur.tiles + sh.item;
     }
     if (!ok && lane == 0) block_attn_error(CF_DEVERR_TIMEOUT);
+    // The CTA that began this item may have told the join of this piece.
+    if (!ok && a.meta != nullptr && cur.tile > 0 && tok < HG) a.part_sum[2 * blockIdx.x * HG + tok] = kNoPiece;
     if (a.meta != nullptr && tok == 0 && !begun) a.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
   }
   tc_fence_before();
@@ -866,7 +871,8 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
 // c + 1 .. last.  With few pieces a warp takes a head, with many (a few rows
 // over all CTAs) the warps share each head's; a lane has the maximum and sum
 // of one of 32 pieces, then its columns of all.
-// out = sum_p w_p o_p / sum_p w_p, w_p = sum_p 2^(max_p - max).
+// out = sum_p w_p o_p / sum_p w_p, w_p = sum_p 2^(max_p - max).  An item with
+// a piece that its CTA could not finish (CF_DEVERR_TIMEOUT) is left unwritten.
 // Latency-bound: three dependent loads (the CTA's entry, the sums, the
 // pieces' outputs) behind a launch that overlaps the streaming kernel's end.
 constexpr int kJoinWarps = 8;
@@ -887,16 +893,19 @@ __global__ void __launch_bounds__(kJoinWarps * 32) block_attention_join_kernel(c
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   T* out = static_cast<T*>(a.out) + ((size_t)meta.x * a.num_heads + kvh * a.group + chunk * HG) * D;
   float m, l, o[E];
+  bool lost;  // a piece
   auto collect = [&](int h, int first, int stride) {  // pieces first, first + stride, ... of head h
     auto slot = [&](int p) { return (size_t)(p == 0 ? 2 * c + 1 : 2 * (c + p)) * HG + h; };
     m = -INFINITY;
     l = 0.f;
+    lost = false;
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.f;
     for (int p0 = first; p0 < pieces; p0 += stride * 32) {
       const int mine = p0 + stride * lane;
       const float sum = mine < pieces ? a.part_sum[slot(mine)] : 0.f;
       const float top = mine < pieces ? a.part_max[slot(mine)] : -INFINITY;
+      lost |= __any_sync(0xffffffffu, sum == kNoPiece) != 0;
       // a piece without a readable token has sum 0
       const float mn = fmaxf(m, warp_max(top));
       const float mu = mn == -INFINITY ? 0.f : mn;
@@ -923,6 +932,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) block_attention_join_kernel(c
   if (pieces <= kFewPieces) {
     for (int h = warp; h < nheads; h += kJoinWarps) {
       collect(h, 0, 1);
+      if (lost) return;
       const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
       for (int e = 0; e < E; ++e) out[h * D + lane * E + e] = from_float<T>(o[e] * inv);
@@ -933,7 +943,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) block_attention_join_kernel(c
     collect(h, warp, kJoinWarps);
     if (lane == 0) {
       sm[warp] = m;
-      sl[warp] = l;
+      sl[warp] = lost ? kNoPiece : l;
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) so[warp][lane * E + e] = o[e];
@@ -945,6 +955,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) block_attention_join_kernel(c
     l = 0.f;
 #pragma unroll
     for (int w = 0; w < kJoinWarps; ++w) {
+      if (sl[w] == kNoPiece) return;  // for the whole block
       scale[w] = exp2f(sm[w] - mu);
       l = fmaf(sl[w], scale[w], l);
     }
@@ -1117,7 +1128,9 @@ cf_status launch_block_scaled_attention(const BlockScaledLaunch& l) {
   a.num_blocks = p.num_blocks;
   const int64_t lim = g_test_wait_limit_ns.load(std::memory_order_relaxed);
   a.wait_limit_ns = lim > 0 ? (uint64_t)lim : kWaitLimitNs;
-  a.unarm_first_stage = g_test_unarm_first_stage.load(std::memory_order_relaxed);
+  a.unarm_cta = g_test_unarm_first_stage.load(std::memory_order_relaxed) != 0
+                    ? g_test_unarm_cta.load(std::memory_order_relaxed)
+                    : kNoCta;
   return dispatch(p, Launch{a, l});
 }
 cf_status block_scaled_read_errors(uint32_t* bits, bool clear) {

@@ -57,6 +57,7 @@ cf_status attention_read_errors(uint32_t* bits, bool clear);
 // Test hooks of the decode kernels' bounded waits (cf_testing_set_pipeline_faults).
 extern std::atomic<int64_t> g_test_wait_limit_ns;
 extern std::atomic<int32_t> g_test_unarm_first_stage;
+extern std::atomic<int32_t> g_test_unarm_cta;
 
 // ---- chunked-prefill attention (prefill_attention.cu) ------------------------
 bool prefill_supported(int32_t head_dim, int32_t block_size, int32_t dtype, int32_t group);

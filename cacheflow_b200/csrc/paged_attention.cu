@@ -1355,6 +1355,7 @@ bool attention_fp8_supported(int32_t head_dim, int32_t block_size, int32_t dtype
 // Test hooks (cf_testing_set_pipeline_faults), read at every launch.
 std::atomic<int64_t> g_test_wait_limit_ns{0};
 std::atomic<int32_t> g_test_unarm_first_stage{0};
+std::atomic<int32_t> g_test_unarm_cta{-1};
 
 cf_status launch_paged_attention(const AttnLaunch& l) {
   const cf_paged_attention_params& p = *l.p;
@@ -1429,5 +1430,11 @@ extern "C" cf_status cf_testing_set_pipeline_faults(int64_t wait_limit_ns, int32
   if (wait_limit_ns < 0 || unarm_first_stage < 0 || unarm_first_stage > 1) return CF_ERR_INVALID_ARGUMENT;
   cfb::g_test_wait_limit_ns.store(wait_limit_ns, std::memory_order_relaxed);
   cfb::g_test_unarm_first_stage.store(unarm_first_stage, std::memory_order_relaxed);
+  return CF_OK;
+}
+
+extern "C" cf_status cf_testing_set_pipeline_fault_cta(int32_t cta) {
+  if (cta < -1) return CF_ERR_INVALID_ARGUMENT;
+  cfb::g_test_unarm_cta.store(cta, std::memory_order_relaxed);
   return CF_OK;
 }

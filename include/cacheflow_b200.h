@@ -520,6 +520,13 @@ CF_API cf_status cf_get_device_errors(int32_t device, uint32_t* flags, int32_t c
  * normal operation.  No counterpart in CacheFlow. */
 CF_API cf_status cf_testing_set_pipeline_faults(int64_t wait_limit_ns, int32_t unarm_first_stage);
 
+/* TEST HOOK: the CTA whose first stage cf_testing_set_pipeline_faults leaves
+ * unarmed in cf_paged_attention_fp8_block_v1 (-1, the default: every CTA), so
+ * that one piece of a context that several CTAs share is not finished.  The
+ * rows that it belongs to are left unwritten, the others are not.  No
+ * counterpart in CacheFlow. */
+CF_API cf_status cf_testing_set_pipeline_fault_cta(int32_t cta);
+
 /* The last cudaError_t seen by any entry point on this thread. */
 CF_API int32_t cf_last_cuda_error(void);
 

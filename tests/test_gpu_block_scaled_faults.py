@@ -1,7 +1,8 @@
 """Decode attention over block-scaled caches when a pipeline wait runs out:
 the call ends, says so, writes no row that it could not finish, and the next
 call is correct.  The waits are made to run out by leaving a CTA's first copies
-out (cf_testing_set_pipeline_faults), with a limit of 1 ms."""
+out (cf_testing_set_pipeline_faults), with a limit of 1 ms
+(20 ms where the other CTAs go on)."""
 
 import contextlib
 import math
@@ -18,14 +19,17 @@ pytestmark = pytest.mark.gpu
 
 
 @contextlib.contextmanager
-def _faults(lib):
+def _faults(lib, cta=-1):
     from cacheflow_b200 import _lib
 
-    assert lib.cf_testing_set_pipeline_faults(1_000_000, 1) == _lib.CF_OK
+    assert lib.cf_testing_set_pipeline_fault_cta(cta) == _lib.CF_OK
+    # where the other CTAs go on, their own waits must not run out
+    assert lib.cf_testing_set_pipeline_faults(1_000_000 if cta < 0 else 20_000_000, 1) == _lib.CF_OK
     try:
         yield
     finally:
         assert lib.cf_testing_set_pipeline_faults(0, 0) == _lib.CF_OK
+        assert lib.cf_testing_set_pipeline_fault_cta(-1) == _lib.CF_OK
 
 
 def _case(dtype, H, Hkv, D, ctx, seed=0):
@@ -90,3 +94,44 @@ def test_every_cta_gives_up(cflib, dtype, H, Hkv, D, workspace):
         assert (got == 7).all() and elapsed < 1.0
     assert _correct(call.run(), want)
     assert ops.device_errors(0) == 0
+
+
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("H", [1, 3, 8, 12])
+def test_one_cta_gives_up(cflib, H, D):
+    """One row's piece is not finished: that row (or the head chunk of it) is
+    left unwritten whatever the workspace holds, the others are as ever.  With
+    no more tiles than CTAs, CTA i has tile i of the rows laid end to end."""
+    from cacheflow_b200 import _lib, ops
+
+    chunks = (H + 7) // 8
+    tiles = [4, 1, 20, 3]  # few pieces, one, many
+    case, want = _case("bf16", H, 1, D, [128 * t - 5 for t in tiles], seed=H)
+    stale = _Call("bf16", case)
+    stale.run()  # leaves pieces of these sizes behind
+    ops.device_errors(0)
+    first = np.cumsum([0] + [t * chunks for t in tiles])
+    for cta in (0, 1, 3, 4 * chunks, 5 * chunks, 5 * chunks + 7, 25 * chunks - 1, 28 * chunks - 1):
+        for values in ("old", 0xFF, 0x3F):
+            call = stale
+            if values != "old":
+                call = _Call("bf16", case, stale=values)
+            with _faults(cflib, cta):
+                got = call.run()
+            assert ops.device_errors(0) & _lib.CF_DEVERR_TIMEOUT
+            row = int(np.searchsorted(first, cta, side="right")) - 1
+            chunk = (cta - first[row]) // tiles[row]
+            lost = slice(8 * chunk, min(H, 8 * chunk + 8))
+            assert (got[row, lost] == 7).all(), (cta, values)
+            keep = np.ones(want.shape[:2], bool)
+            keep[row, lost] = False
+            assert _correct(got[keep], want[keep]), (cta, values)
+    assert _correct(stale.run(), want)
+    assert ops.device_errors(0) == 0
+
+
+def test_hook_checks_its_argument(cflib):
+    from cacheflow_b200 import _lib
+
+    assert cflib.cf_testing_set_pipeline_fault_cta(-2) == _lib.CF_ERR_INVALID_ARGUMENT
+    assert cflib.cf_testing_set_pipeline_fault_cta(-1) == _lib.CF_OK
