@@ -1078,17 +1078,25 @@ cf_status launch_block(BlockArgs b, bool interleaved, cudaStream_t stream) {
   const RopeArgs& a = b.r;
   const int windows = (a.num_tokens + kBlk - 1) / kBlk;
   // Two CTAs per SM are resident.  Up to a CTA per SM a window's heads are
-  // shared among several, and the Q rows take what is left of one wave; once
-  // the windows are more than that, Q rows get up to four CTAs per SM among
-  // them (1024 decode rows of 64 / 8 heads 18 us, 28 with the others' rule;
-  // 16384 tokens of 32 / 8 heads 126 us, 131 with eight, 152 with two, before
-  // the search took what it takes now).
+  // shared among several.  The Q rows take what the windows leave of one wave
+  // as long as a Q CTA is done with them about when the windows are, which
+  // take as long as 4 rounds of Q items and 3.7 for each KB of a token's K.
+  // Past that they get up to four CTAs per SM among the windows.  Measured,
+  // one wave / four per SM: 32 / 8 heads of 128, 2048 tokens 21 / 28 us, 3400
+  // (10 rounds) 33 / 36, 3600 (13) 40 / 37, 4096 75 / 40; 64 / 8 heads, 2400 (8)
+  // 28 / 37, 3200 (17) 52 / 45; 128 / 8 heads, 1600 (8) 29 / 39, 2368 (16) 51 / 48;
+  // 32 / 8 of 256, 3200 (17) 54 / 67, 3600 (25) 76 / 75; 32 / 32, 4200 (32) 81 / 91,
+  // 4300 (40) 111 / 94; 12 / 4 of 96, 3600 (6) 24 / 26, 4000 (11) 37 / 27.  Two or
+  // eight per SM in place of four: 16384 tokens of 32 / 8 heads 128 and 119 / 117.
   const int sms = sm_count();
   const int split = sms / windows;
   b.head_split = split < 1 ? 1 : (split > a.num_kv_heads ? a.num_kv_heads : split);
   b.kv_ctas = windows * b.head_split;
-  const int64_t cap = b.kv_ctas <= sms ? 2 * sms - b.kv_ctas : 4 * (int64_t)sms;
-  b.q_ctas = a.num_heads > 0 ? (int32_t)row_ctas(a, K == 1 ? 4 : 1, kWarps, cap, {a.num_heads}) : 0;
+  const int64_t left = 2 * (int64_t)sms - b.kv_ctas;
+  constexpr int U = K == 1 ? 4 : 1;
+  const double rounds = 4 + 3.7 / 1024 * a.num_kv_heads * a.head_dim * (double)sizeof(T);
+  const bool one_wave = left > 0 && row_ctas(a, U, kWarps, INT32_MAX, {a.num_heads}) <= rounds * left;
+  b.q_ctas = a.num_heads > 0 ? (int32_t)row_ctas(a, U, kWarps, one_wave ? left : 4 * (int64_t)sms, {a.num_heads}) : 0;
   const unsigned grid = (unsigned)(b.kv_ctas + b.q_ctas);
   if constexpr (K == 1) {
     if (full_rows(a))
