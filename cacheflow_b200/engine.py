@@ -42,6 +42,11 @@ class Rotation(NamedTuple):
     interleaved: bool = False
 
 
+def _block_scales(x, cache: torch.Tensor) -> bool:
+    """Whether x is meant as scales for each block and KV head; a tensor of one number is a whole cache's."""
+    return isinstance(x, torch.Tensor) and (x.numel() > 1 or (x.dim() == 2 and x.shape == cache.shape[:2]))
+
+
 class _Slot:
     def __init__(self, max_seqs, max_new, num_heads, num_kv_heads, head_dim, max_blocks, dt, dev, max_chunks):
         self.q = torch.empty((max_seqs, num_heads, head_dim), dtype=dt, device=dev)
@@ -79,9 +84,19 @@ class DecodeEngine:
         if kernel not in ("v1", "reference"):
             raise ValueError("kernel must be 'v1' or 'reference'")
         self.rotation = rotation
-        self.block_scaled = kv_scales is not None and isinstance(kv_scales[0], torch.Tensor) and kv_scales[0].dim() == 2
-        if self.block_scaled and (kernel != "v1" or fused_append or key_cache.dtype != torch.float8_e4m3fn):
-            raise ValueError("block scales: float8_e4m3fn caches, kernel='v1', fused_append=False")
+        self.block_scaled = kv_scales is not None and any(_block_scales(x, key_cache) for x in kv_scales)
+        if self.block_scaled:
+            # before anything is appended that could not be attended to
+            if kernel != "v1" or fused_append or key_cache.dtype != torch.float8_e4m3fn:
+                raise ValueError("block scales: float8_e4m3fn caches, kernel='v1', fused_append=False")
+            if key_cache.shape[2] != 16 or key_cache.shape[3] not in (128, 256) \
+                    or query_dtype not in (torch.float16, torch.bfloat16):
+                raise ValueError("block scales: blocks of 16 tokens, head_dim 128 or 256, query_dtype f16 or bf16")
+            if len(kv_scales) != 2 or any(not isinstance(x, torch.Tensor) or x.dtype != torch.float32
+                                          or x.shape != key_cache.shape[:2] or x.device != key_cache.device
+                                          or not x.is_contiguous() for x in kv_scales):
+                raise ValueError("block scales: two contiguous float32 tensors [num_blocks, num_kv_heads] on the "
+                                 "caches' device")
         if rotation is not None and fused_append:
             raise ValueError("a rotation appends in its own launch: fused_append=False")
         self.k = key_cache
