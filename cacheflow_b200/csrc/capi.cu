@@ -245,6 +245,8 @@ cf_status check_rope_params(const cf_rope_params* p, bool with_cache) {
   return CF_OK;
 }
 
+bool aligned4(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
+
 // The block-scaled caches' shapes.
 cf_status check_block_cache(int32_t head_dim, int32_t block_size, int64_t num_blocks) {
   if (block_size <= 0 || num_blocks <= 0) return CF_ERR_INVALID_ARGUMENT;
@@ -469,7 +471,8 @@ cf_status cf_rope_and_cache(const cf_rope_params* p, void* key_cache, void* valu
   if (p->num_tokens == 0) return CF_OK;
   if (!key_cache || !value_cache || !slot_mapping) return CF_ERR_INVALID_ARGUMENT;
   const uintptr_t eb = dtype_bytes(p->dtype);
-  if (reinterpret_cast<uintptr_t>(key_cache) % eb || reinterpret_cast<uintptr_t>(value_cache) % eb)
+  if (reinterpret_cast<uintptr_t>(key_cache) % eb || reinterpret_cast<uintptr_t>(value_cache) % eb ||
+      !aligned4(slot_mapping))
     return CF_ERR_INVALID_ARGUMENT;
   return launch_rope_and_cache(*p, key_cache, value_cache, slot_mapping, block_size, num_blocks, false, 1.f,
                                1.f, (cudaStream_t)stream);
@@ -486,7 +489,8 @@ cf_status cf_rope_and_cache_fp8(const cf_rope_params* p, void* key_cache, void* 
     return CF_ERR_INVALID_ARGUMENT;
   if (p->head_dim % 16 != 0) return CF_ERR_UNSUPPORTED;
   if (p->num_tokens == 0) return CF_OK;
-  if (!key_cache || !value_cache || !slot_mapping || !aligned16(key_cache) || !aligned16(value_cache))
+  if (!key_cache || !value_cache || !slot_mapping || !aligned16(key_cache) || !aligned16(value_cache) ||
+      !aligned4(slot_mapping))
     return CF_ERR_INVALID_ARGUMENT;
   return launch_rope_and_cache(*p, key_cache, value_cache, slot_mapping, block_size, num_blocks, true,
                                k_scale, v_scale, (cudaStream_t)stream);
@@ -501,7 +505,7 @@ cf_status cf_rope_and_cache_fp8_block(const cf_rope_params* p, void* key_cache, 
   st = check_block_cache(p->head_dim, block_size, num_blocks);
   if (st != CF_OK || p->num_tokens == 0) return st;
   if (!key_cache || !value_cache || !k_scales || !v_scales || !slot_mapping || !aligned16(key_cache) ||
-      !aligned16(value_cache))
+      !aligned16(value_cache) || !aligned4(k_scales) || !aligned4(v_scales) || !aligned4(slot_mapping))
     return CF_ERR_INVALID_ARGUMENT;
   return launch_rope_and_cache_fp8_block(*p, key_cache, value_cache, k_scales, v_scales, slot_mapping,
                                          num_blocks, (cudaStream_t)stream);
@@ -524,7 +528,7 @@ cf_status cf_reshape_and_cache_fp8_block(const void* key, const void* value, voi
     return CF_ERR_INVALID_ARGUMENT;
   const uintptr_t eb = dtype_bytes(dtype);
   if (reinterpret_cast<uintptr_t>(key) % eb || reinterpret_cast<uintptr_t>(value) % eb || !aligned16(key_cache) ||
-      !aligned16(value_cache))
+      !aligned16(value_cache) || !aligned4(k_scales) || !aligned4(v_scales) || !aligned4(slot_mapping))
     return CF_ERR_INVALID_ARGUMENT;
   cf_rope_params p = {};
   p.key = key;
@@ -554,6 +558,8 @@ cf_status cf_paged_attention_fp8_block_v1(const cf_paged_attention_params* p, co
   if (st != CF_OK) return st;
   if ((st = check_fp8(p, 1.f, 1.f)) != CF_OK || p->num_seqs == 0) return st;
   if (!k_scales || !v_scales || p->num_blocks <= 0) return CF_ERR_INVALID_ARGUMENT;
+  if (!aligned4(k_scales) || !aligned4(v_scales) || !aligned4(p->block_tables) || !aligned4(p->context_lens))
+    return CF_ERR_INVALID_ARGUMENT;
   // TMA rows and token counts are int32
   if (p->num_blocks > INT32_MAX / p->block_size / p->num_kv_heads || p->max_blocks_per_seq > (INT32_MAX - 128) / 16)
     return CF_ERR_UNSUPPORTED;
