@@ -524,7 +524,7 @@ def reshape_and_cache_fp8_block(key, value, key_cache, value_cache, k_scales, v_
 
 
 def paged_attention_fp8_block_workspace_size(query, key_cache, block_tables, max_context_len) -> int:
-    """Bytes of optional workspace that lets paged_attention_fp8_block_v1 split long contexts."""
+    """Bytes of optional workspace that lets paged_attention_fp8_block_v1 split long contexts on query's device."""
     lib = _lib.load()
     p = AttentionParams()
     p.num_seqs = query.shape[0]
@@ -533,7 +533,12 @@ def paged_attention_fp8_block_workspace_size(query, key_cache, block_tables, max
     p.max_context_len = int(max_context_len)
     p.max_blocks_per_seq = block_tables.shape[1]
     p.dtype = dtype_code(query.dtype)
-    return int(lib.cf_paged_attention_fp8_block_workspace_size(ctypes.byref(p)))
+    # the split goes by the device's multiprocessors
+    dev = query.get_device()
+    if dev < 0 or dev == torch.cuda.current_device():
+        return int(lib.cf_paged_attention_fp8_block_workspace_size(ctypes.byref(p)))
+    with torch.cuda.device(dev):
+        return int(lib.cf_paged_attention_fp8_block_workspace_size(ctypes.byref(p)))
 
 
 def paged_attention_fp8_block_v1(out, query, key_cache, value_cache, k_scales, v_scales, block_tables, context_lens,
