@@ -802,8 +802,7 @@ def run_ours(args):
                            for name in args.side_configs.split(",") if name != args.workload}
     if rank == 0:
         if world == 1 and not args.no_cpu_baseline:
-            line["cpu_baseline"] = cpu_baseline(w, budget_s=args.cpu_seconds)
-            line["cpu_port"] = cpu_port_baseline(w)
+            line.update(cpu_baselines(w, args.cpu_seconds))
         print(json.dumps(line), flush=True)
     if world > 1:
         dist.barrier()
@@ -906,6 +905,11 @@ def cpu_baseline(w: workloads.Workload, budget_s: float = 15.0, steps: int | Non
     }
 
 
+def no_reference(e: FileNotFoundError) -> str:
+    """Why CacheFlow's own step cannot be timed, in one line."""
+    return f"the reference's CPU build, made from its sources, is not here: {e}"
+
+
 def cpu_port_baseline(w: workloads.Workload, max_seqs: int = 16, max_tokens: int = 2048,
                       budget_s: float = 4.0) -> dict:
     """The oracle's C restatement of the decode step (correct softmax
@@ -950,6 +954,15 @@ def cpu_port_baseline(w: workloads.Workload, max_seqs: int = 16, max_tokens: int
     }
 
 
+def cpu_baselines(w: workloads.Workload, budget_s: float) -> dict:
+    """The line's host baselines: CacheFlow's own step where its build is here, and the oracle's."""
+    try:
+        ref = cpu_baseline(w, budget_s=budget_s)
+    except FileNotFoundError as e:
+        ref = {"unavailable": no_reference(e)}
+    return {"cpu_baseline": ref, "cpu_port": cpu_port_baseline(w)}
+
+
 def run_reference(args):
     rank, world, local = dist_env()
     if rank != 0:
@@ -959,7 +972,11 @@ def run_reference(args):
     seqs_total = workloads.make(args.workload, seed=1234,
                                 **({"num_seqs": args.num_seqs} if args.num_seqs else {})).num_seqs \
         if scaling == "strong" else w.num_seqs * world
-    cb = cpu_baseline(w, steps=args.steps, warmup=args.warmup, total_budget_s=args.cpu_total_seconds)
+    try:
+        cb = cpu_baseline(w, steps=args.steps, warmup=args.warmup, total_budget_s=args.cpu_total_seconds)
+    except FileNotFoundError as e:
+        print(json.dumps({"impl": "reference", "unavailable": no_reference(e)}), flush=True)
+        return
     line = {
         "metric": METRIC,
         "value": cb["value"],
