@@ -697,7 +697,10 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
       const int cnt = cur.count();
       const int kvh = cur.item / a.head_chunks, chunk = cur.item - kvh * a.head_chunks;
       float qsc[HG], m[HG], l[HG], beta[HG], acc[L::kBoxes][HG];
-      if (warp == 0 && !wait_bar(q_full, (uint32_t)seg & 1u, a.wait_limit_ns)) fail[0] = 1;
+      if (warp == 0) {
+        if (!wait_bar(q_full, (uint32_t)seg & 1u, a.wait_limit_ns)) fail[0] = 1;
+        __syncwarp();  // lanes may have given up at different tries; a warp meets as one
+      }
       ok = meet(0);
       if (!ok) break;
 #pragma unroll
@@ -727,9 +730,12 @@ __global__ void __launch_bounds__(kThreads, Layout<T, D, HG>::kMinCtas)
       };
       for (int i = 0; i < cnt; ++i, ++j) {
         const int par = (int)(j & 1), s = (int)(j % S);
-        if (warp == 0 && !(wait_bar(&v_full[s], (j / S) & 1u, a.wait_limit_ns) &&
-                           wait_bar(&s_full[par], (j >> 1) & 1u, a.wait_limit_ns)))
-          fail[1] = 1;
+        if (warp == 0) {
+          if (!(wait_bar(&v_full[s], (j / S) & 1u, a.wait_limit_ns) &&
+                wait_bar(&s_full[par], (j >> 1) & 1u, a.wait_limit_ns)))
+            fail[1] = 1;
+          __syncwarp();
+        }
         ok = meet(1);
         if (!ok) break;
         tc_fence_after();
