@@ -121,8 +121,8 @@ struct Cursor {
 // but for tokens that next to nothing is left for in their tile.  The sum L
 // has the weights before they are rounded.  With the row's running maximum as
 // the reference the rest of a row with one dominant token fell under that
-// floor as a whole (131072 tokens with 1 % of the weight beside one: 60-84 %
-// of the output lost).
+// floor as a whole (131072 tokens with at most 1 % of the weight beside one
+// whose values are zeros: by its roundings 84 % of the output lost).
 //
 // Roles: warps 4 and 5 issue the TMA copies of K and of V (2 KB boxes of 16
 // tokens x 128 bytes, 128-byte swizzle) into rings of stages, warp 7 stages
@@ -136,11 +136,15 @@ struct Cursor {
 // they wait for each other's maxima.
 //
 // Bound: HBM, the caches' bytes.  Measured, of 6.54 TB/s that a copy reaches:
-// 16 rows of 16384-131072 tokens, 32 / 8 heads, bf16, 291 us, 6.36 TB/s; 256
-// rows of 512-8192, 64 / 8 heads, 247 us, 5.94 TB/s; 64 rows of 128-4096, 32 /
-// 32 heads, f16, 103 us, 5.9 TB/s; one row of 1001 tokens 10.4 us, the chain of
-// one tile and the join.  What is left at many rows is the 8 us to the first
-// tile, shares that end apart, and the join.
+// 16 rows of 16384-131072 tokens, 32 / 8 heads, bf16, 291 us, 6.37 TB/s; 256
+// rows of 512-8192, 64 / 8 heads, 251 us, 5.84 TB/s at 1965 MHz (calls in a row
+// and replayed graphs alike; run for seconds, at the card's power cap and 1650-
+// 1800 MHz, both take 271-280, since the softmax has half of the issue slots);
+// 64 rows of 128-4096, 32 / 32 heads, f16, 103 us, 5.9 TB/s;
+// one row of 1001 tokens 10.4 us, the chain of one tile and the join.  What is
+// left at many rows is the 8 us to the first tile, shares that end apart, and
+// the join.  Groups past 8 heads read K and V once for each chunk: see
+// dispatch().
 // ---------------------------------------------------------------------------
 constexpr int kThreads = 256;  // two warpgroups: softmax, and the rest
 constexpr int kKWarp = 4;
@@ -154,8 +158,10 @@ constexpr float kNoMax = -3.402823466e38f;  // the maximum over no token: finite
 // among it), so that L, which counts weights over their vs, stays in range.
 constexpr float kLeastScale = 8.67361737988403547e-19f;
 
-// e4m3 terms of a query element and of a weight: two hold a bf16's 8
-// significant bits, three an f16's 11.
+// e4m3 terms of a query element and of a weight: while they are normal, two
+// hold a bf16's 8 significant bits, three an f16's 11.  More terms for a weight
+// would take its floor down (four bits each) and cost the softmax warps the
+// time of f16's third: with 8 heads 62 us against 55 (64 rows of 512-4096, 64 / 8 heads).
 template <typename T>
 constexpr int kTerms = std::is_same<T, __half>::value ? 3 : 2;
 
@@ -1075,9 +1081,12 @@ cf_status launch_heads(Args a, const BlockScaledLaunch& l) {
 }
 
 // Calls f with the kernel's types as template arguments: HG query heads of a
-// KV head per item, larger groups in chunks of 8 (16 heads in one item left
-// room for two CTAs per SM: 64 rows of 1024-8192 tokens 89 us, 83 as two
-// items, whose KV bytes meet in L2).
+// KV head per item, larger groups in chunks of 8.  Chunks are items of their
+// own, so each reads the KV head's K and V: from L2 where they are still
+// there (64 rows of 1024-8192 tokens, 4 KV heads, 16 heads each, 83 us; 89 as
+// one item, which leaves room for two CTAs per SM), from HBM where rows are
+// long and many (64 rows of 8192 tokens, 8 KV heads: 2.18 GB read with 16
+// heads each, 1.09 GB with 8; 256 such rows 1321 and 662 us).
 template <typename F>
 auto dispatch(const cf_paged_attention_params& p, F&& f) {
   const int group = p.num_heads / p.num_kv_heads;

@@ -501,7 +501,9 @@ def reshape_and_cache_fp8_block(key, value, key_cache, value_cache, k_scales, v_
     block's scale is the smallest power of two that its rows need (max |x| <=
     448 scale); a call that writes the block's offset 0 starts it over, any
     other one raises the scale where its rows need it and stores the rows that
-    are there anew.  Scales move with their blocks: copy_blocks and the other
+    are there anew.  Rows of a block may come in any order; of two tokens with
+    one slot the later is stored.  More than 16384 tokens count as consecutive
+    calls of 16384.  Scales move with their blocks: copy_blocks and the other
     block operators take scales.view(num_blocks, num_kv_heads, 1, 1).
     """
     lib = _lib.load()
@@ -546,7 +548,8 @@ def paged_attention_fp8_block_v1(out, query, key_cache, value_cache, k_scales, v
                                  workspace: torch.Tensor | None = None) -> torch.Tensor:
     """Decode attention over float8_e4m3fn caches whose blocks have a scale for each KV head (K = k_scales[block,
     head] * stored, V alike; as reshape_and_cache_fp8_block fills them); query and output f16 or bf16, head_dim 128
-    or 256.  The workspace (paged_attention_fp8_block_workspace_size bytes) lets long contexts split."""
+    or 256.  The workspace (paged_attention_fp8_block_workspace_size bytes) lets long contexts split.  A weight times
+    its V scale is held to 2^-8 of itself (f16 2^-11), or to 2^-22 (2^-26) of the largest among its 128 neighbours."""
     lib = _lib.load()
     qs, cs, bs = query.shape, key_cache.shape, block_tables.shape
     if len(qs) != 3 or len(cs) != 4 or len(bs) != 2 or out.shape != qs or value_cache.shape != cs or cs[3] != qs[2] \

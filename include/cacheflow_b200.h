@@ -371,8 +371,9 @@ CF_API cf_status cf_rope_and_cache_fp8(const cf_rope_params* params, void* key_c
  * power-of-two scales the division is exact and storing rows anew loses
  * nothing but what falls under e4m3's smallest normal.  A new pool's scales
  * start at 0; one that is not a positive finite number counts as 0.  Rows of a block may come in any order and place of the call;
- * of two tokens with one slot the later is stored (calls of more than 16384
- * tokens count as consecutive calls of 16384).  The scale arrays move with
+ * of two tokens with one slot the later is stored.  Calls of more than 16384
+ * tokens count as consecutive calls of 16384: the one that holds a block's
+ * offset 0 starts it over, also after rows that an earlier one wrote.  The scale arrays move with
  * their blocks: cf_copy_blocks and the other block operators take them as
  * caches of block_size 1, head_dim 1, CF_F32.
  * key, value [num_tokens, num_kv_heads, head_dim] of `dtype` (CF_F32, CF_F16
